@@ -401,7 +401,9 @@ def work(case):
     if case["op"] == "norm_fwd":
         tensors = 3 + (case["output_norm"] != "none")
         return {"bytes": tensors * size * entries + 4 * n * vectors + 16 * tokens, "flops": 14 * entries + generator}
-    return {"bytes": 6 * size * entries + 8 * n * vectors + 16 * tokens, "flops": 32 * entries + generator}
+    # dy, dh, h in, two gradients out; the block's output is needed for its norm and for the gate's gradient only
+    tensors = 5 + (case["branch_norm"] != "none" or case["gates"] > 0)
+    return {"bytes": tensors * size * entries + 8 * n * vectors + 16 * tokens, "flops": 32 * entries + generator}
 
 
 # ---------------------------------------------------------------- the same from the definitions, in 64 bits
