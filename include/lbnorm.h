@@ -714,6 +714,191 @@ int lbn_batch_norm_bwd_f64(lbn_stream_t stream, int64_t channels, int64_t channe
                            double* dmean, double* dvar,
                            void* workspace, size_t workspace_bytes);
 
+/* --------------------------------------------------- dropout (counter-based generator)
+ * The forward and backward of a dropout layer with keep probability `keep_prob` (0 < keep_prob
+ * <= 1; 1 copies): y = kept ? x / q : 0, dx = kept ? dy / q : 0, with the same entries kept in
+ * both directions.  Nothing is stored between them: whether entry (r, c) is kept is a function
+ * of (seed, offset, r, column_offset + c) alone.  The generator is Philox-4x32 with ten rounds
+ * (Salmon, Moraes, Dror, Shaw, SC11): key = seed (low word first), counter = (r / 8,
+ * column_offset + c, offset low, offset high); entry r of a column takes the sixteen bits
+ * number r % 8 of the four output words (word (r % 8) / 2, low half for even r) and is kept if
+ * they are below t = floor(65536 keep_prob + 1/2), at least 1.  q = t / 65536, so outputs are
+ * unbiased.  Pass another `offset` for every call (a step or layer counter), and in
+ * column_offset the global index of the call's first column when a mini-batch is cut.  step
+ * (device, may be NULL): a counter that is added to `offset` when the kernel runs, for calls
+ * that are recorded into a graph and must not repeat their mask: advance it between replays,
+ * and leave it as it was in forward until backward has run.  Dropped entries are 0 whatever x holds.
+ * x and y (dy and dx) may be the same matrix.  fp32, IEEE binary16 or bfloat16 storage, fp32
+ * arithmetic.  LBN_ERR_UNSUPPORTED beyond 2^34 rows or 2^32 columns (column_offset included). */
+int lbn_dropout_fwd_f32(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const float* x, int64_t ldx, float* y, int64_t ldy);
+int lbn_dropout_fwd_f16(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const void* x, int64_t ldx, void* y, int64_t ldy);
+int lbn_dropout_fwd_bf16(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const void* x, int64_t ldx, void* y, int64_t ldy);
+int lbn_dropout_bwd_f32(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const float* dy, int64_t lddy, float* dx, int64_t lddx);
+int lbn_dropout_bwd_f16(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const void* dy, int64_t lddy, void* dx, int64_t lddx);
+int lbn_dropout_bwd_bf16(lbn_stream_t stream, int64_t height, int64_t width, double keep_prob,
+                        uint64_t seed, uint64_t offset, const uint64_t* step, int64_t column_offset,
+                        const void* dy, int64_t lddy, void* dx, int64_t lddx);
+
+/* --------------------------------------------------------------------- residual norm
+ * A transformer's residual stream between two blocks.  For column t (a token) of `size`
+ * features, o = branch (the block's output), r = residual (the stream):
+ *     u = N1(o);  v = kept ? u / q : 0;  h = residual_multiplier r + branch_multiplier g v;
+ *     y = N2(h)
+ * N1 (branch_norm, after the block) and N2 (output_norm, before the next one) are each
+ * LBN_NORM_NONE, LBN_NORM_RMS (v rsqrt(mean(v^2) + epsilon) scale + bias) or LBN_NORM_LAYER
+ * ((v - mean) rsqrt(var + epsilon) scale + bias, biased variance).  Dropout is that of
+ * lbn_dropout_* with the same arguments and the same mask (keep_prob 1: none).
+ *   residual: NULL for no stream (r = 0).   gate: fp32 matrix of num_gates columns; column t
+ *   uses gate column t / (width / num_gates): 1 for one learned gate, the number of samples for
+ *   one gate per sample, `width` for a full gate; num_gates 0 and NULL for none.  width must be a
+ *   multiple of num_gates.
+ *   branch_scale, branch_bias, output_scale, output_bias: fp32 vectors of `size`, NULL for 1 resp.
+ *   0; must be NULL where the norm is LBN_NORM_NONE.
+ *   h: the new stream, NULL if not wanted.  y: NULL exactly if output_norm is LBN_NORM_NONE
+ *   (then h is required).  y is formed from h before h is rounded to its storage type.
+ *   stats: (4 x width) fp32: mean and variance of o, mean and variance of h (RMS: 0 and the mean of
+ *   squares; no norm: 0 and 1), kept for backward; NULL if not wanted (inference).
+ * Outputs may take the place of inputs of the same shape and leading dimension (h that of r or
+ * o, y likewise).  Storage fp32, IEEE binary16 or bfloat16; arithmetic, statistics, weights,
+ * gates and their gradients fp32. */
+#define LBN_NORM_NONE 0
+#define LBN_NORM_RMS 1
+#define LBN_NORM_LAYER 2
+int lbn_residual_norm_fwd_f32(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const float* branch, int64_t ld_branch,
+                              const float* residual, int64_t ld_residual, const float* gate,
+                              int64_t ld_gate, int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale,
+                              const float* output_bias, double keep_prob, uint64_t seed,
+                              uint64_t offset, const uint64_t* step, int64_t column_offset,
+                              float* h, int64_t ld_h, float* y, int64_t ld_y, float* stats,
+                              int64_t ld_stats);
+int lbn_residual_norm_fwd_f16(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const void* branch, int64_t ld_branch,
+                              const void* residual, int64_t ld_residual, const float* gate,
+                              int64_t ld_gate, int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale,
+                              const float* output_bias, double keep_prob, uint64_t seed,
+                              uint64_t offset, const uint64_t* step, int64_t column_offset,
+                              void* h, int64_t ld_h, void* y, int64_t ld_y, float* stats,
+                              int64_t ld_stats);
+int lbn_residual_norm_fwd_bf16(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const void* branch, int64_t ld_branch,
+                              const void* residual, int64_t ld_residual, const float* gate,
+                              int64_t ld_gate, int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale,
+                              const float* output_bias, double keep_prob, uint64_t seed,
+                              uint64_t offset, const uint64_t* step, int64_t column_offset,
+                              void* h, int64_t ld_h, void* y, int64_t ld_y, float* stats,
+                              int64_t ld_stats);
+/* Backward.  dy = dL/dy (NULL exactly if output_norm is LBN_NORM_NONE), dh = dL/dh as far as it
+ * does not come through y (NULL: zero; required without an output norm); h (required with an output norm),
+ * stats and the dropout arguments as forward left and took them; branch is read (and
+ * required) only with a branch norm or a gate gradient.  dbranch = dL/do, dresidual = dL/dr
+ * (NULL: not wanted), both may take the place of dy, dh, h or branch of the same leading
+ * dimension.  dgate (size x num_gates), dbranch_scale, dbranch_bias, doutput_scale,
+ * doutput_bias: overwritten where non-NULL (NULL: not wanted; must be NULL for a norm that is
+ * LBN_NORM_NONE, dgate without a gate).
+ * The workspace is lbn_residual_norm_bwd_workspace_bytes() large, 16-byte aligned:
+ * has_weight_grads != 0 if any of the four weight gradients is wanted, num_gate_grads =
+ * num_gates if dgate is, else 0, elem_bytes 4 or 2 for the storage type. */
+size_t lbn_residual_norm_bwd_workspace_bytes(int64_t size, int64_t width, int has_weight_grads,
+                                             int64_t num_gate_grads, int elem_bytes);
+int lbn_residual_norm_bwd_f32(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const float* branch, int64_t ld_branch,
+                              const float* h, int64_t ld_h, const float* gate, int64_t ld_gate,
+                              int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale, double keep_prob,
+                              uint64_t seed, uint64_t offset, const uint64_t* step,
+                              int64_t column_offset, const float* stats, int64_t ld_stats,
+                              const float* dy, int64_t ld_dy, const float* dh, int64_t ld_dh,
+                              float* dbranch, int64_t ld_dbranch, float* dresidual,
+                              int64_t ld_dresidual, float* dgate, int64_t ld_dgate,
+                              float* dbranch_scale, float* dbranch_bias, float* doutput_scale,
+                              float* doutput_bias, void* workspace, size_t workspace_bytes);
+int lbn_residual_norm_bwd_f16(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const void* branch, int64_t ld_branch,
+                              const void* h, int64_t ld_h, const float* gate, int64_t ld_gate,
+                              int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale, double keep_prob,
+                              uint64_t seed, uint64_t offset, const uint64_t* step,
+                              int64_t column_offset, const float* stats, int64_t ld_stats,
+                              const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,
+                              void* dbranch, int64_t ld_dbranch, void* dresidual,
+                              int64_t ld_dresidual, float* dgate, int64_t ld_dgate,
+                              float* dbranch_scale, float* dbranch_bias, float* doutput_scale,
+                              float* doutput_bias, void* workspace, size_t workspace_bytes);
+int lbn_residual_norm_bwd_bf16(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,
+                              int output_norm, float epsilon, float residual_multiplier,
+                              float branch_multiplier, const void* branch, int64_t ld_branch,
+                              const void* h, int64_t ld_h, const float* gate, int64_t ld_gate,
+                              int64_t num_gates, const float* branch_scale,
+                              const float* branch_bias, const float* output_scale, double keep_prob,
+                              uint64_t seed, uint64_t offset, const uint64_t* step,
+                              int64_t column_offset, const float* stats, int64_t ld_stats,
+                              const void* dy, int64_t ld_dy, const void* dh, int64_t ld_dh,
+                              void* dbranch, int64_t ld_dbranch, void* dresidual,
+                              int64_t ld_dresidual, float* dgate, int64_t ld_dgate,
+                              float* dbranch_scale, float* dbranch_bias, float* doutput_scale,
+                              float* doutput_bias, void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------- logits adjustment
+ * What a decoding step does to the logits of `width` sequences (one column of `vocabulary`
+ * entries each) before the softmax layer.  For entry v of column s, c = how often v is among the generated
+ * tokens, seen = v occurs in the prompt or among them:
+ *     z = x_v;  if seen: z = z > 0 ? z / repetition[s] : z * repetition[s]
+ *     z = z - (frequency[s] c + (c > 0 ? presence[s] : 0)) + bias_v
+ *     y_v = the grammar allows v ? z : -infinity
+ *   tokens: int32 matrix of max_tokens rows, the history of a sequence in its column: the first
+ *   prompt_lengths[s] are the prompt, those up to lengths[s] were generated (lengths NULL: all
+ *   max_tokens; prompt_lengths NULL: 0; values beyond [0, max_tokens] are clamped).  Tokens outside
+ *   [0, vocabulary) count for nothing, and so do places behind the length, whatever they hold.
+ *   repetition, presence, frequency: one fp32 value per sequence, NULL for 1, 0, 0.
+ *   bias_tokens, bias_values: num_biases entries per sequence; tokens outside the vocabulary are
+ *   unused places; of several entries for one token the last one holds.
+ *   mask: num_masks columns of 32-bit words, bit v % 32 of word v / 32 set = v is allowed; sequence
+ *   s uses column mask_index[s] (negative: no grammar; num_masks or more: nothing is allowed),
+ *   without mask_index column s (num_masks == width) or the only one.
+ * A grammar that allows nothing leaves a column of -infinity, on which the softmax layers
+ * return NaN: end such a sequence first.  x and y may be the same matrix.  No workspace.
+ * Storage fp32, IEEE binary16 or bfloat16, fp32 arithmetic, one rounding. */
+int lbn_logits_adjust_f32(lbn_stream_t stream, int64_t vocabulary, int64_t width, const float* x,
+                          int64_t ldx, float* y, int64_t ldy, const int32_t* tokens, int64_t ld_tokens,
+                          int64_t max_tokens, const int32_t* lengths, const int32_t* prompt_lengths,
+                          const float* repetition, const float* presence, const float* frequency,
+                          const int32_t* bias_tokens, int64_t ld_bias_tokens, const float* bias_values,
+                          int64_t ld_bias_values, int64_t num_biases, const uint32_t* mask,
+                          int64_t ld_mask, int64_t num_masks, const int32_t* mask_index);
+int lbn_logits_adjust_f16(lbn_stream_t stream, int64_t vocabulary, int64_t width, const void* x,
+                          int64_t ldx, void* y, int64_t ldy, const int32_t* tokens, int64_t ld_tokens,
+                          int64_t max_tokens, const int32_t* lengths, const int32_t* prompt_lengths,
+                          const float* repetition, const float* presence, const float* frequency,
+                          const int32_t* bias_tokens, int64_t ld_bias_tokens, const float* bias_values,
+                          int64_t ld_bias_values, int64_t num_biases, const uint32_t* mask,
+                          int64_t ld_mask, int64_t num_masks, const int32_t* mask_index);
+int lbn_logits_adjust_bf16(lbn_stream_t stream, int64_t vocabulary, int64_t width, const void* x,
+                          int64_t ldx, void* y, int64_t ldy, const int32_t* tokens, int64_t ld_tokens,
+                          int64_t max_tokens, const int32_t* lengths, const int32_t* prompt_lengths,
+                          const float* repetition, const float* presence, const float* frequency,
+                          const int32_t* bias_tokens, int64_t ld_bias_tokens, const float* bias_values,
+                          int64_t ld_bias_values, int64_t num_biases, const uint32_t* mask,
+                          int64_t ld_mask, int64_t num_masks, const int32_t* mask_index);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,7 @@ f64 = ctypes.c_double
 cint = ctypes.c_int
 vp = ctypes.c_void_p
 sz = ctypes.c_size_t
+u64 = ctypes.c_uint64
 
 LBN_OK = 0
 LBN_ERR_INVALID_ARGUMENT = -1
@@ -22,6 +23,9 @@ LBN_ERR_UNSUPPORTED = -3
 LBN_STATS_TWO_PASS = 0
 LBN_STATS_SUMSQ = 1
 LBN_STATS_REFERENCE_ORDER = 2
+LBN_NORM_NONE = 0
+LBN_NORM_RMS = 1
+LBN_NORM_LAYER = 2
 
 # name -> (restype, argtypes); mirrors include/lbnorm.h declaration by declaration
 PROTOTYPES = {
@@ -120,7 +124,20 @@ PROTOTYPES = {
                                       vp, vp, vp, vp, vp, sz, cint]),
     "lbn_batch_norm_bwd_f64": (cint, [vp, i64, i64, i64, cint, f64, cint, vp, i64, vp, i64, vp, i64, vp,
                                       vp, vp, vp, vp, vp, vp, vp, vp, vp, sz]),
+    "lbn_residual_norm_bwd_workspace_bytes": (sz, [i64, i64, cint, i64, cint]),
 }
+# the operators that exist for fp32, fp16 and bfloat16 storage with the same arguments
+for _t in ("f32", "f16", "bf16"):
+    for _d in ("fwd", "bwd"):
+        PROTOTYPES[f"lbn_dropout_{_d}_{_t}"] = (cint, [vp, i64, i64, f64, u64, u64, vp, i64, vp, i64, vp, i64])
+    PROTOTYPES[f"lbn_residual_norm_fwd_{_t}"] = (
+        cint, [vp, i64, i64, cint, cint, f32, f32, f32, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, f64, u64, u64,
+               vp, i64, vp, i64, vp, i64, vp, i64])
+    PROTOTYPES[f"lbn_residual_norm_bwd_{_t}"] = (
+        cint, [vp, i64, i64, cint, cint, f32, f32, f32, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, f64, u64, u64, vp,
+               i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, vp, sz])
+    PROTOTYPES[f"lbn_logits_adjust_{_t}"] = (
+        cint, [vp, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, i64, vp, i64, i64, vp, i64, i64, vp])
 
 _lib = None
 

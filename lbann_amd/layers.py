@@ -1,6 +1,7 @@
 """Host-side mirror of the LBANN layer classes (layer norm, batch norm, softmax, log-softmax,
 channelwise softmax; instance norm, entry-wise batch norm, cross entropy and the two scale/bias
-layers), over the C ABI.
+layers) and of the operators around a transformer's residual stream and logits (dropout,
+residual norm, logits adjustment), over the C ABI.
 
 Each class keeps the reference layer's constructor parameters, its member
 matrices and its two compute hooks, `fp_compute()` and `bp_compute()`
@@ -41,6 +42,19 @@ class DeviceMatrix:
         if fill is not None:
             self.tensor.fill_(fill)
 
+    @classmethod
+    def attach(cls, tensor, height):
+        """View of a (width, ldim) tensor that someone else owns (El::Matrix::Attach); no copy."""
+        if tensor.dim() != 2 or tensor.shape[1] < height or (tensor.shape[1] > 1 and tensor.stride(1) != 1):
+            raise ValueError("attach takes a (width, ldim) tensor whose columns are contiguous and hold `height` entries")
+        m = cls.__new__(cls)
+        m.height, m.width = int(height), tensor.shape[0]
+        m.ldim = int(tensor.stride(0)) if tensor.shape[0] > 1 else max(tensor.shape[1], 1)
+        if m.ldim < m.height:
+            raise ValueError("attach: columns overlap")
+        m.tensor = tensor
+        return m
+
     # El::Matrix vocabulary
     def Height(self):
         return self.height
@@ -79,7 +93,7 @@ class DeviceMatrix:
         workgroups that ran out in any call since the last check raises ClusterWaitTimedOut."""
         check_cluster_waits()
         t = self.tensor[: self.width, : self.height]
-        if t.dtype == torch.float16:
+        if t.dtype in (torch.float16, torch.bfloat16):
             t = t.float()
         return np.asfortranarray(t.cpu().numpy().T)
 
@@ -765,6 +779,279 @@ def softmax_cross_entropy_backward(softmax, cross_entropy, dloss, want_dtruth=Fa
          dtruth.ldim if dtruth is not None else 0, ws, nb)
     _after_call()
     return dx
+
+
+_SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+
+
+def _suffix_of(m):
+    try:
+        return _SUFFIX[m.dtype]
+    except KeyError:
+        raise TypeError(f"storage is fp32, fp16 or bfloat16, not {m.dtype}") from None
+
+
+def _same_kind(like, height, width, **matrices):
+    """Every given matrix has the shape, the storage type and the device of `like`."""
+    for name, m in matrices.items():
+        if m is not None and ((m.height, m.width) != (height, width) or m.dtype != like.dtype
+                              or m.tensor.device != like.tensor.device):
+            raise ValueError(f"{name} is {m.height} x {m.width} {m.dtype} on {m.tensor.device}; expected "
+                             f"{height} x {width} {like.dtype} on {like.tensor.device}")
+
+
+def _on_current_device(m):
+    """Kernels go to the current stream of the current device: refuse matrices of another one."""
+    if m.tensor.device.type != "cuda" or m.tensor.device.index != torch.cuda.current_device():
+        raise ValueError(f"matrix on {m.tensor.device}; the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def _buffer(m):
+    """(address, leading dimension) of an optional matrix."""
+    return (None, 0) if m is None else (m.tensor.data_ptr(), m.ldim)
+
+
+def _device_values(t, n, dtype, what, like):
+    """Address of an optional device vector of at least n entries."""
+    if t is None:
+        return None
+    t = getattr(t, "tensor", t)
+    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (n > 1 and t.stride(0) != 1) or t.device != like.tensor.device:
+        raise ValueError(f"{what}: expected {n} contiguous {dtype} values on {like.tensor.device}")
+    return t.data_ptr()
+
+
+class _Dropout:
+    """Where the random bits of a layer's calls come from: key `seed`, counter `offset`.  Every
+    training-mode forward without an explicit offset takes the next one."""
+
+    def __init__(self, keep_prob, seed):
+        if not 0.0 < keep_prob <= 1.0:
+            raise ValueError(f"keep_prob is {keep_prob}; it must be in (0, 1]")
+        self.m_keep_prob = float(keep_prob)
+        self.m_seed = int(seed) & 0xFFFFFFFFFFFFFFFF
+        self.m_offset = 0           # of the last forward, which backward repeats
+        self.m_column_offset = 0    # global index of the first column of this process's mini-batch
+        self.m_step = None          # int64 device tensor of one value added to the offset when a kernel runs
+        self.m_kept = 1.0           # keep probability of the last forward (1 outside training)
+        self._next = 0
+
+    def _start(self, training, offset):
+        if offset is None and training and self.m_keep_prob < 1.0:
+            offset = self._next
+            self._next = offset + 1 & 0xFFFFFFFFFFFFFFFF
+        if offset is not None:
+            self.m_offset = int(offset) & 0xFFFFFFFFFFFFFFFF
+        self.m_kept = self.m_keep_prob if training else 1.0
+
+    def _drop_args(self, like):
+        step = None
+        if self.m_step is not None:
+            step = _device_values(self.m_step, 1, torch.int64, "m_step", like)
+        return self.m_kept, self.m_seed, self.m_offset, step, self.m_column_offset
+
+
+class dropout_layer(_Layer, _Dropout):
+    """Dropout (LBANN's dropout layer: include/lbann/layers/regularizers/dropout.hpp) from a
+    counter-based generator: the mask is a function of (seed, offset, row, column) and is never
+    stored; backward forms it again."""
+
+    def __init__(self, keep_prob=0.5, seed=0, device="cuda"):
+        _Layer.__init__(self, device)
+        _Dropout.__init__(self, keep_prob, seed)
+        self.m_kept = self.m_keep_prob
+
+    def forward(self, x, in_place=False, training=True, offset=None):
+        self._start(training, offset)
+        return super().forward(x, in_place)
+
+    def _call(self, direction, x, y):
+        _same_kind(x, x.height, x.width, output=y)
+        _on_current_device(x)
+        return (f"lbn_dropout_{direction}_{_suffix_of(x)}",
+                (_stream(), x.height, x.width, *self._drop_args(x), *_buffer(x), *_buffer(y)))
+
+    def fp_call(self):
+        return self._call("fwd", self.prev_activations, self.activations)
+
+    def bp_call(self):
+        return self._call("bwd", self.prev_error_signals, self.error_signals)
+
+
+class residual_norm_layer(_Dropout):
+    """The residual stream between two transformer blocks in one call each way:
+
+        u = N1(branch);  v = dropout(u);  h = a * residual + b * gate * v;  y = N2(h)
+
+    with N1 (`branch_norm`) and N2 (`output_norm`) "none", "rms" or "layer".  scale / bias arguments
+    are arrays or device tensors of `size` fp32 values, None for no such weight; scales default
+    to one where a norm is chosen and `None` is given.  branch, residual, h and y share one
+    storage type: fp32, fp16 or bfloat16.
+
+    forward(branch, residual, gate) returns y (None without an output norm) and keeps the new
+    stream in `residual`; backward(dy, dresidual) returns (dbranch, dresidual of the old stream)
+    and leaves the weights' gradients in m_{branch,output}_{scale,bias}_gradient and
+    m_gate_gradient."""
+
+    KINDS = {"none": capi.LBN_NORM_NONE, "rms": capi.LBN_NORM_RMS, "layer": capi.LBN_NORM_LAYER}
+
+    def __init__(self, size, branch_norm="none", output_norm="rms", epsilon=1e-5, residual_multiplier=1.0,
+                 branch_multiplier=1.0, branch_scale=None, branch_bias=None, output_scale=None, output_bias=None,
+                 keep_prob=1.0, seed=0, device="cuda"):
+        super().__init__(keep_prob, seed)
+        for kind in (branch_norm, output_norm):
+            if kind not in self.KINDS:
+                raise ValueError(f"unknown norm {kind!r}; expected one of {sorted(self.KINDS)}")
+        self.device = device
+        self.size = int(size)
+        self.m_branch_norm, self.m_output_norm = branch_norm, output_norm
+        self.m_epsilon = float(epsilon)
+        self.m_residual_multiplier, self.m_branch_multiplier = float(residual_multiplier), float(branch_multiplier)
+        self._kinds = self.KINDS[branch_norm], self.KINDS[output_norm]
+        self.weights = {}
+        for name, value, kind in (("branch_scale", branch_scale, branch_norm), ("branch_bias", branch_bias, branch_norm),
+                                  ("output_scale", output_scale, output_norm), ("output_bias", output_bias, output_norm)):
+            if value is None:
+                self.weights[name] = None
+            elif kind == "none":
+                raise ValueError(f"{name} without a norm to scale")
+            else:
+                t = value if isinstance(value, torch.Tensor) else torch.as_tensor(np.asarray(value, np.float32))
+                self.weights[name] = t.to(device=device, dtype=torch.float32).contiguous()
+                if t.dim() != 1 or t.numel() != self.size:
+                    raise ValueError(f"{name} has shape {tuple(t.shape)}; expected ({self.size},)")
+        self.branch = self.h = self.gate = self.residual = self.activations = self.m_statistics = None
+        self.m_has_residual = False
+        self.m_gate_gradient = None
+        for name in self.weights:
+            setattr(self, f"m_{name}_gradient", None)
+
+    def _new(self, like, width, height=None, dtype=None):
+        return DeviceMatrix(self.size if height is None else height, width, dtype=dtype or like.dtype,
+                            device=like.tensor.device)
+
+    def _check_gate(self, gate, like):
+        if gate is None:
+            return
+        if gate.height != self.size or gate.width < 1 or like.width % gate.width or gate.dtype != torch.float32 \
+                or gate.tensor.device != like.tensor.device:
+            raise ValueError(f"gate is {gate.height} x {gate.width} {gate.dtype}; expected {self.size} rows of fp32 on "
+                             f"{like.tensor.device} and a number of columns that divides {like.width}")
+
+    def forward(self, branch, residual=None, gate=None, training=True, offset=None, in_place=False):
+        """in_place: the new stream overwrites `residual` and y overwrites `branch` (inference: backward
+        needs what they held).  training=False: no dropout, no statistics."""
+        _same_kind(branch, self.size, branch.width, branch=branch, residual=residual)
+        _on_current_device(branch)
+        self._check_gate(gate, branch)
+        self._start(training, offset)
+        w = branch.width
+        self.branch, self.gate, self.m_has_residual = branch, gate, residual is not None
+        stream_out = residual if in_place and residual is not None else self._new(branch, w)
+        y = None
+        if self._kinds[1]:
+            y = branch if in_place else self._new(branch, w)
+        self.m_statistics = self._new(branch, w, 4, torch.float32) if training else None
+        wt = self.weights
+        call(f"lbn_residual_norm_fwd_{_suffix_of(branch)}", _stream(), self.size, w, *self._kinds, self.m_epsilon,
+             self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch), *_buffer(residual), *_buffer(gate),
+             gate.width if gate is not None else 0, _pointer(wt["branch_scale"]), _pointer(wt["branch_bias"]),
+             _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch), *_buffer(stream_out),
+             *_buffer(y), *_buffer(self.m_statistics))
+        self.h = self.residual = stream_out
+        self.activations = y
+        return y
+
+    def bind_saved(self, branch, h, statistics, gate=None, has_residual=True, offset=0, training=True):
+        """What an earlier forward left behind, for a backward without one in this object
+        (recomputation, pipelines): its block output, new stream, statistics, gate and dropout offset."""
+        self._check_gate(gate, h)
+        self.branch, self.h, self.m_statistics, self.gate = branch, h, statistics, gate
+        self.residual, self.m_has_residual = h, bool(has_residual)
+        self._start(training, offset)
+
+    def backward(self, dy=None, dresidual=None):
+        like = dy if dy is not None else dresidual
+        if like is None or (dy is not None) != bool(self._kinds[1]):
+            raise ValueError("backward takes dy exactly if there is an output norm, and dresidual if there is none")
+        if self.m_statistics is None:
+            raise ValueError("backward needs a training-mode forward (or bind_saved) first")
+        w = like.width
+        _same_kind(like, self.size, w, dy=dy, dresidual=dresidual, branch=self.branch, h=self.h)
+        if (self.m_statistics.height, self.m_statistics.width, self.m_statistics.dtype) != (4, w, torch.float32):
+            raise ValueError("the statistics are a (4 x width) fp32 matrix")
+        _on_current_device(like)
+        dbranch = self._new(like, w)
+        dres = self._new(like, w) if self.m_has_residual else None
+        wt, kinds = self.weights, self._kinds
+        for name, t in wt.items():
+            setattr(self, f"m_{name}_gradient", None if t is None else _Vector(self.size, like.tensor.device))
+        gate = self.gate
+        self.m_gate_gradient = None if gate is None else DeviceMatrix(self.size, gate.width, device=like.tensor.device)
+        grads = [getattr(self, f"m_{name}_gradient") for name in ("branch_scale", "branch_bias", "output_scale", "output_bias")]
+        gates = gate.width if gate is not None else 0
+        need = capi.lib().lbn_residual_norm_bwd_workspace_bytes(
+            self.size, w, int(any(g is not None for g in grads)), gates, like.tensor.element_size())
+        # scratch of this call alone: nothing that another stream or a recorded graph could share
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=like.tensor.device)
+        call(f"lbn_residual_norm_bwd_{_suffix_of(like)}", _stream(), self.size, w, *kinds, self.m_epsilon,
+             self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(self.branch),
+             *(_buffer(self.h) if kinds[1] else (None, 0)), *_buffer(gate), gates, _pointer(wt["branch_scale"]),
+             _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), *self._drop_args(like), *_buffer(self.m_statistics),
+             *_buffer(dy), *_buffer(dresidual), *_buffer(dbranch), *_buffer(dres), *_buffer(self.m_gate_gradient),
+             *(_pointer(None if g is None else g.tensor) for g in grads), ws.data_ptr(), need)
+        return dbranch, dres
+
+
+class logits_adjust_layer:
+    """Penalties for repeated tokens, bias lists and grammar masks on the logits of a decoding
+    step, in front of the softmax layer.  One column per sequence; see lbn_logits_adjust_* in
+    include/lbnorm.h for the formula.  Forward only."""
+
+    def __init__(self, vocabulary, device="cuda"):
+        self.vocabulary = int(vocabulary)
+        self.device = device
+        self.activations = None
+
+    @staticmethod
+    def _matrix(m, width, dtype, what, like, height=None):
+        if m is None:
+            return None, 0, 0
+        if m.dtype != dtype or m.tensor.device != like.tensor.device or (width is not None and m.width != width) \
+                or (height is not None and m.height != height):
+            raise ValueError(f"{what} is {m.height} x {m.width} {m.dtype} on {m.tensor.device}")
+        return m.tensor.data_ptr(), m.ldim, m.height
+
+    def forward(self, x, tokens=None, lengths=None, prompt_lengths=None, repetition=None, presence=None, frequency=None,
+                bias_tokens=None, bias_values=None, mask=None, mask_index=None, in_place=False):
+        """x: (vocabulary x sequences).  tokens: (max_tokens x sequences) int32, lengths and
+        prompt_lengths int32 vectors; repetition, presence, frequency fp32 vectors; bias_tokens
+        (int32) and bias_values (fp32): (entries x sequences); mask: (ceil(vocabulary / 32) x
+        grammars) int32 words, mask_index an int32 vector.  Everything but x is optional."""
+        w = x.width
+        _same_kind(x, self.vocabulary, w, logits=x)
+        _on_current_device(x)
+        y = x if in_place else DeviceMatrix(self.vocabulary, w, dtype=x.dtype, device=x.tensor.device)
+        if (bias_tokens is None) != (bias_values is None):
+            raise ValueError("bias_tokens and bias_values go together")
+        words = (self.vocabulary + 31) // 32
+        tok, ld_tok, max_tokens = self._matrix(tokens, w, torch.int32, "tokens", x)
+        bt, ld_bt, biases = self._matrix(bias_tokens, w, torch.int32, "bias_tokens", x)
+        bv, ld_bv, _ = self._matrix(bias_values, w, torch.float32, "bias_values", x, biases or None)
+        mk, ld_mk, _ = self._matrix(mask, None, torch.int32, "mask", x, words)
+        call(f"lbn_logits_adjust_{_suffix_of(x)}", _stream(), self.vocabulary, w, *_buffer(x), *_buffer(y), tok, ld_tok,
+             max_tokens, _device_values(lengths, w, torch.int32, "lengths", x),
+             _device_values(prompt_lengths, w, torch.int32, "prompt_lengths", x),
+             _device_values(repetition, w, torch.float32, "repetition", x),
+             _device_values(presence, w, torch.float32, "presence", x),
+             _device_values(frequency, w, torch.float32, "frequency", x), bt, ld_bt, bv, ld_bv, biases, mk, ld_mk,
+             mask.width if mask is not None else 0, _device_values(mask_index, w, torch.int32, "mask_index", x))
+        self.activations = y
+        return y
 
 
 class gradient_buffer:
