@@ -21,7 +21,7 @@
 // grows from one pair to the next and no row is used twice.
 #include "device_utils.hpp"
 #include "host_utils.hpp"
-#include "residual_norm_long.hpp"
+#include "residual_norm_rows.hpp"
 
 namespace lbn {
 
@@ -86,6 +86,34 @@ static bool rn_ld_ok(const void* p, int64_t ld, int64_t height, int64_t width) {
 
 static bool rn_norm_ok(int kind) { return kind >= kNormNone && kind <= kNormLayer; }
 
+// How a column is shared: V units of eight entries per thread, a team of 16 lanes (`sub`) or of nw
+// waves.  v == 0: it does not fit `max_v` units per thread of a full workgroup.
+struct RnShape {
+  int v, nw;
+  bool sub;
+  int threads() const { return sub || nw == 1 ? 256 : kWave * nw; }
+  int teams() const { return sub ? 16 : (nw == 1 ? 4 : 1); }
+};
+
+static RnShape rn_shape(int64_t n, int max_v)
+{
+  const int64_t units = ceil_div(n, 8);
+  if (units <= 16) return {1, 1, true};
+  if (units <= 32) return {2, 1, true};
+  for (int v = 1; v <= max_v; v *= 2)
+    if (units <= 1024 * v) return {v, static_cast<int>(ceil_div(units, kWave * v)), false};
+  return {0, 0, false};
+}
+
+template <typename T, int V, bool SUB>
+static void rn_launch_fwd(hipStream_t st, const RnFwdArgs<T>& a, const RnShape& shape)
+{
+  const int64_t blocks = ceil_div(a.width, shape.teams());
+  const int64_t resident = resident_blocks(rn_fwd_rows<T, V, SUB>, shape.threads());
+  const int64_t grid = resident > 0 && blocks > resident ? resident : (blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30));
+  hipLaunchKernelGGL((rn_fwd_rows<T, V, SUB>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads()), 0, st, a, shape.nw);
+}
+
 template <typename T>
 static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double keep_prob, uint64_t seed,
                   uint64_t offset, const uint64_t* step, int64_t column_offset)
@@ -107,8 +135,15 @@ static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double
   a.cols_per_gate = num_gates > 0 ? a.width / num_gates : a.width;
   a.drop = drop_args(keep_prob, seed, offset, step, column_offset);
   hipStream_t st = as_stream(stream);
-  const int64_t grid = a.width < (int64_t(1) << 30) ? a.width : (int64_t(1) << 30);
-  hipLaunchKernelGGL((rn_fwd_long<T>), dim3(static_cast<unsigned>(grid)), dim3(kRnLongThreads), 0, st, a);
+  const RnShape shape = rn_shape(a.n, 2);
+  switch (shape.v) {
+  case 1: shape.sub ? rn_launch_fwd<T, 1, true>(st, a, shape) : rn_launch_fwd<T, 1, false>(st, a, shape); break;
+  case 2: shape.sub ? rn_launch_fwd<T, 2, true>(st, a, shape) : rn_launch_fwd<T, 2, false>(st, a, shape); break;
+  default: {
+    const int64_t grid = a.width < (int64_t(1) << 30) ? a.width : (int64_t(1) << 30);
+    hipLaunchKernelGGL((rn_fwd_long<T>), dim3(static_cast<unsigned>(grid)), dim3(kRnLongThreads), 0, st, a);
+  }
+  }
   return launch_status();
 }
 

@@ -1,0 +1,283 @@
+// Residual norm, the kernels that hold a column in registers: every tensor crosses HBM once.
+//
+// A "unit" is eight consecutive entries of a column, what one counter of the generator serves;
+// a thread owns V units.  A team works on a column: 16 lanes (a DPP row) for up to 128 V
+// features, otherwise NW whole waves, 512 V NW >= n; a workgroup holds several teams where a team
+// is at most a wave, else one.  Teams walk columns with the next column's loads in flight and,
+// for V = 1, the weights of their units in registers.
+//
+// One norm costs one workgroup barrier: a wave takes the mean and the squared deviations of its own
+// entries from registers (two passes, no E[x^2] - mean^2 cancellation), and the pairs of the
+// waves are merged as sums over parts are:  M2 = sum of M2_w + n_w (mean_w - mean)^2.
+#pragma once
+
+#include "residual_norm_long.hpp"
+
+namespace lbn {
+
+template <typename T>
+struct Unit {
+  typedef T raw_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  static __device__ __forceinline__ raw_t load(const T* p, int valid)
+  {
+    if (valid == 8) return *reinterpret_cast<const raw_t*>(p);
+    raw_t r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = j < valid ? p[j] : static_cast<T>(0.f);
+    return r;
+  }
+  static __device__ __forceinline__ void widen(const raw_t& r, float (&v)[8])
+  {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(r[j]);
+  }
+};
+
+// Which entries of its column a thread owns: unit(i) = t + i * lanes, valid[i] of its entries exist.
+template <int V>
+struct RowShare {
+  int unit[V], valid[V];
+  __device__ __forceinline__ RowShare(int t, int lanes, int n)
+  {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      unit[i] = t + i * lanes;
+      const int left = n - 8 * unit[i];
+      valid[i] = left < 0 ? 0 : (left > 8 ? 8 : left);
+    }
+  }
+};
+
+template <bool SUB>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+  return SUB ? row16_sum(v) : wave_sum(v);
+}
+
+// Merges over the waves of a team (one team per workgroup when nw > 1).
+struct TeamMerge {
+  float2 (*slots)[16];  // two buffers, zero behind wave nw
+  int nw, wave, lane;
+  float count;          // entries of the column that wave (lane % 16) owns
+  int turn = 0;
+
+  __device__ __forceinline__ float2 exchange(float a, float b)
+  {
+    if (lane == 0) slots[turn][wave] = make_float2(a, b);
+    __syncthreads();
+    const float2 r = slots[turn][lane & 15];
+    turn ^= 1;  // the other buffer's barrier separates two uses of this one
+    return r;
+  }
+  __device__ __forceinline__ void sum2(float& a, float& b)
+  {
+    const float2 r = exchange(a, b);
+    a = row16_sum(r.x);
+    b = row16_sum(r.y);
+  }
+};
+
+// Mean and variance of a column from registers.  Entries that do not exist do not count.
+template <int V, bool SUB, bool FULL>
+__device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowShare<V>& share, int kind, float inv_n,
+                                            float inv_mine, TeamMerge& merge, float& mean, float& var)
+{
+  float part_mean = 0.f;
+  if (kind == kNormLayer) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += FULL || j < share.valid[i] ? x[i][j] : 0.f;
+    part_mean = lanes_sum<SUB>(s) * inv_mine;
+  }
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = FULL || j < share.valid[i] ? x[i][j] - part_mean : 0.f;
+      q = __builtin_fmaf(d, d, q);
+    }
+  q = lanes_sum<SUB>(q);
+  mean = part_mean;
+  if (!SUB && merge.nw > 1) {
+    const float2 r = merge.exchange(part_mean, q);
+    if (kind == kNormLayer) {
+      mean = row16_sum(merge.count * r.x) * inv_n;
+      const float d = r.x - mean;
+      q = row16_sum(__builtin_fmaf(merge.count * d, d, r.y));
+    }
+    else {
+      q = row16_sum(r.y);
+    }
+  }
+  var = q * inv_n;
+}
+
+// What a team needs to know about itself; block-wide set-up of the merge buffers included.
+template <int V, bool SUB>
+struct Team {
+  int index, per_block, t;
+  float inv_n, inv_mine;  // 1 / entries of the column, of this wave
+  __device__ __forceinline__ Team(int nw, int n, float2 (*slots)[16], TeamMerge& merge)
+  {
+    const int tid = threadIdx.x;
+    const int lanes = SUB ? 16 : kWave * nw;
+    per_block = static_cast<int>(blockDim.x) / lanes;
+    index = SUB ? tid / 16 : wave_index() / nw;
+    t = tid - index * lanes;
+    merge.slots = slots;
+    merge.nw = nw;
+    merge.lane = tid & (kWave - 1);
+    merge.wave = SUB ? 0 : wave_index() - index * nw;
+    auto entries_of = [&](int wave) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int left = n - 8 * (wave * kWave + i * lanes);
+        c += left < 0 ? 0 : (left > 8 * kWave ? 8 * kWave : left);
+      }
+      return c;
+    };
+    inv_n = 1.f / static_cast<float>(n);
+    inv_mine = inv_n;
+    merge.count = 0.f;
+    if (!SUB) {
+      const int mine = entries_of(merge.wave);
+      inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f;
+      merge.count = (merge.lane & 15) < nw ? static_cast<float>(entries_of(merge.lane & 15)) : 0.f;
+      if (nw > 1) {
+        if (tid < 32) slots[tid >> 4][tid & 15] = make_float2(0.f, 0.f);
+        __syncthreads();
+      }
+    }
+  }
+};
+
+template <typename T, int V, bool SUB>
+__global__ void __launch_bounds__(SUB ? 256 : 1024)
+rn_fwd_rows(RnFwdArgs<T> a, int nw)
+{
+  using U = Unit<T>;
+  constexpr bool kKeepWeights = V == 1 || SUB;  // of a thread's units, in registers from column to column
+  constexpr bool kPrefetch = V == 1 || SUB;
+  constexpr int WV = kKeepWeights ? V : 1;
+  __shared__ float2 slots[2][16];
+  TeamMerge merge;
+  const int n = static_cast<int>(a.n);
+  const Team<V, SUB> team(nw, n, slots, merge);
+  const RowShare<V> share(team.t, SUB ? 16 : kWave * nw, n);
+  const DropStream stream = drop_stream(a.drop);
+  const bool dropping = a.drop.threshold < 65536u;
+  const bool one_gate = a.gate && a.cols_per_gate == a.width;
+
+  auto gate_of = [&](int64_t col) { return a.gate ? a.gate + col / a.cols_per_gate * a.ld_gate : nullptr; };
+  auto weights = [&](const float* w, int i, float fill, float (&out)[8]) {
+    load_weights8(w, 8 * share.unit[i], share.valid[i], fill, out);
+  };
+  float w1[WV][8], b1[WV][8], w2[WV][8], b2[WV][8], gt[WV][8];
+  if constexpr (kKeepWeights) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      weights(a.branch_scale, i, 1.f, w1[i]);
+      weights(a.branch_bias, i, 0.f, b1[i]);
+      weights(a.output_scale, i, 1.f, w2[i]);
+      weights(a.output_bias, i, 0.f, b2[i]);
+      weights(one_gate ? a.gate : nullptr, i, 1.f, gt[i]);
+    }
+  }
+
+  typename U::raw_t qo[V], qr[V];
+  auto issue = [&](int64_t col) {
+    const T* o = a.branch + col * a.ld_branch;
+#pragma unroll
+    for (int i = 0; i < V; ++i) qo[i] = U::load(o + 8 * share.unit[i], share.valid[i]);
+    if (a.residual) {
+      const T* r = a.residual + col * a.ld_residual;
+#pragma unroll
+      for (int i = 0; i < V; ++i) qr[i] = U::load(r + 8 * share.unit[i], share.valid[i]);
+    }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * team.per_block;
+
+  // full: every unit of every thread exists, nothing is masked
+  auto walk = [&](auto full) {
+    constexpr bool kFull = decltype(full)::value;
+    int64_t col = static_cast<int64_t>(blockIdx.x) * team.per_block + team.index;
+    if (kPrefetch && col < a.width) issue(col);
+    for (; col < a.width; col += step) {
+      if (!kPrefetch) issue(col);
+      float x[V][8], r[V][8];
+#pragma unroll
+      for (int i = 0; i < V; ++i) U::widen(qo[i], x[i]);
+      if (a.residual) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) U::widen(qr[i], r[i]);
+      }
+      if (kPrefetch && col + step < a.width) issue(col + step);
+      if (a.gate && !one_gate && kKeepWeights) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) weights(gate_of(col), i, 1.f, gt[i]);
+      }
+      float mean1 = 0.f, var1 = 1.f, mean2 = 0.f, var2 = 1.f;
+      if (a.branch_norm != kNormNone) {
+        row_moments<V, SUB, kFull>(x, share, a.branch_norm, team.inv_n, team.inv_mine, merge, mean1, var1);
+        const float rstd = rn_rstd(var1 + a.epsilon);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if constexpr (!kKeepWeights) {
+            weights(a.branch_scale, i, 1.f, w1[0]);
+            weights(a.branch_bias, i, 0.f, b1[0]);
+          }
+          constexpr bool kw = kKeepWeights;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[i][j] = __builtin_fmaf((x[i][j] - mean1) * rstd, w1[kw ? i : 0][j], b1[kw ? i : 0][j]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (dropping) {
+          uint32_t w[4];
+          drop_words(a.drop, stream, share.unit[i], static_cast<uint32_t>(col), w);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[i][j] = drop_kept(w, j, a.drop.threshold) ? x[i][j] * a.drop.inverse_keep : 0.f;
+        }
+        if constexpr (!kKeepWeights) weights(gate_of(col), i, 1.f, gt[0]);
+        constexpr bool kw = kKeepWeights;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[i][j] *= a.branch_mult * gt[kw ? i : 0][j];
+          if (a.residual) x[i][j] = __builtin_fmaf(a.residual_mult, r[i][j], x[i][j]);
+        }
+        if (a.h) store8(a.h + col * a.ld_h + 8 * share.unit[i], share.valid[i], x[i]);
+      }
+      if (a.output_norm != kNormNone) {
+        row_moments<V, SUB, kFull>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
+        const float rstd = rn_rstd(var2 + a.epsilon);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if constexpr (!kKeepWeights) {
+            weights(a.output_scale, i, 1.f, w2[0]);
+            weights(a.output_bias, i, 0.f, b2[0]);
+          }
+          constexpr bool kw = kKeepWeights;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            x[i][j] = __builtin_fmaf((x[i][j] - mean2) * rstd, w2[kw ? i : 0][j], b2[kw ? i : 0][j]);
+          store8(a.y + col * a.ld_y + 8 * share.unit[i], share.valid[i], x[i]);
+        }
+      }
+      if (a.stats && team.t == 0) {
+        float* st = a.stats + col * a.ld_stats;
+        st[0] = mean1, st[1] = var1, st[2] = mean2, st[3] = var2;
+      }
+    }
+  };
+  if (n == 8 * V * (SUB ? 16 : kWave * nw)) walk(std::true_type{});
+  else walk(std::false_type{});
+}
+
+}  // namespace lbn
