@@ -33,53 +33,42 @@ struct RnMergeArgs {
   int64_t n, ranges, ld_dgate, num_gates, cols_per_gate, cols_per_range;
 };
 
-__global__ void __launch_bounds__(256)
+// A workgroup sums kMergeLanes neighbouring features: kMergeGroups groups of lanes take every
+// kMergeGroups-th partial row, then a tree over the groups, all in a fixed order.
+constexpr int kMergeLanes = 64, kMergeGroups = 16;
+
+__global__ void __launch_bounds__(kMergeLanes * kMergeGroups)
 rn_merge(RnMergeArgs a)
 {
-  const int64_t k = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (k >= a.n) return;
+  __shared__ float sums[kMergeGroups][kMergeLanes];
+  const int lane = threadIdx.x % kMergeLanes, group = threadIdx.x / kMergeLanes;
+  const int64_t k = static_cast<int64_t>(blockIdx.x) * kMergeLanes + lane;
   for (int64_t item = blockIdx.y; item < kGradGate + a.num_gates; item += gridDim.y) {
     const int q = item < kGradGate ? static_cast<int>(item) : kGradGate;
     if (!a.out[q]) continue;
-    if (q < kGradGate) {
-      float s = 0.f;
-      for (int64_t b = 0; b < a.ranges; ++b) s += a.part[q][b * a.n + k];
-      a.out[q][k] = s;
+    const int64_t gate = item - kGradGate;  // the partial rows from `first` to `last`
+    int64_t first = 0, last = a.ranges - 1;
+    float* out = a.out[q];
+    if (q == kGradGate) {
+      first = gate * a.cols_per_gate / a.cols_per_range;
+      last = ((gate + 1) * a.cols_per_gate - 1) / a.cols_per_range;
+      if (first == last) continue;  // written by the range that holds it
+      first += gate, last += gate;
+      out += gate * a.ld_dgate;
     }
-    else {
-      const int64_t gate = item - kGradGate;
-      const int64_t first = gate * a.cols_per_gate / a.cols_per_range;
-      const int64_t last = ((gate + 1) * a.cols_per_gate - 1) / a.cols_per_range;
-      float s = 0.f;
-      for (int64_t b = first; b <= last; ++b) s += a.part[q][(b + gate) * a.n + k];
-      a.out[q][gate * a.ld_dgate + k] = s;
+    float s = 0.f;
+    if (k < a.n)
+      for (int64_t b = first + group; b <= last; b += kMergeGroups) s += a.part[q][b * a.n + k];
+    sums[group][lane] = s;
+    __syncthreads();
+#pragma unroll
+    for (int half = kMergeGroups / 2; half > 0; half /= 2) {
+      if (group < half) sums[group][lane] += sums[group + half][lane];
+      __syncthreads();
     }
+    if (group == 0 && k < a.n) out[k] = sums[0][lane];
+    __syncthreads();
   }
-}
-
-// Ranges of columns that leave partial rows of their own.
-static int64_t rn_ranges(int64_t width)
-{
-  const int64_t per = ceil_div(width, width < 256 ? width : 256);
-  return ceil_div(width, per);
-}
-
-struct RnBwdPlan {
-  int64_t ranges, cols_per_range;
-  size_t sums_bytes, weight_bytes, gate_bytes;
-  size_t total() const { return sums_bytes + weight_bytes + gate_bytes; }
-};
-
-static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t gate_grads)
-{
-  RnBwdPlan p{};
-  p.cols_per_range = ceil_div(width, rn_ranges(width));
-  p.ranges = ceil_div(width, p.cols_per_range);
-  auto round16 = [](int64_t b) { return static_cast<size_t>(ceil_div(b, 16) * 16); };
-  p.sums_bytes = round16(width * 16);
-  if (weight_grads) p.weight_bytes = round16(kGradGate * p.ranges * n * 4);
-  if (gate_grads) p.gate_bytes = round16((p.ranges + gate_grads) * n * 4);
-  return p;
 }
 
 static bool rn_ld_ok(const void* p, int64_t ld, int64_t height, int64_t width) { return !p || width <= 1 || ld >= height; }
@@ -103,6 +92,63 @@ static RnShape rn_shape(int64_t n, int max_v)
   for (int v = 1; v <= max_v; v *= 2)
     if (units <= 1024 * v) return {v, static_cast<int>(ceil_div(units, kWave * v)), false};
   return {0, 0, false};
+}
+
+// Backward: how many ranges of columns leave partial rows, and how a range is worked on.
+struct RnBwdPlan {
+  RnShape shape;  // v == 0: the long kernels
+  int teams;
+  int64_t ranges, cols_per_range;
+  size_t sums_bytes, weight_bytes, gate_bytes;
+  size_t total() const { return sums_bytes + weight_bytes + gate_bytes; }
+};
+
+static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t gate_grads)
+{
+  RnBwdPlan p{};
+  p.shape = rn_shape(n, 1);
+  constexpr int64_t kRanges = 256;  // one workgroup per compute unit
+  if (p.shape.v == 1) {
+    // a workgroup of up to 8 waves (16 for the widest teams), as many teams as leave a column for every workgroup
+    const int64_t most = p.shape.sub ? 32 : (p.shape.nw <= 8 ? 8 / p.shape.nw : 1);
+    p.teams = static_cast<int>(most);
+    while (p.teams > (p.shape.sub ? 4 : 1) && width < kRanges * p.teams) p.teams = p.shape.sub ? p.teams / 2 : p.teams - 1;
+  }
+  else {
+    p.shape.v = 0;
+    p.teams = 1;
+  }
+  p.cols_per_range = ceil_div(width, kRanges);
+  if (p.cols_per_range < p.teams) p.cols_per_range = p.teams;
+  p.ranges = ceil_div(width, p.cols_per_range);
+  auto round16 = [](int64_t b) { return static_cast<size_t>(ceil_div(b, 16) * 16); };
+  p.sums_bytes = p.shape.v ? 0 : round16(width * 16);
+  if (weight_grads) p.weight_bytes = round16(kGradGate * p.ranges * n * 4);
+  if (gate_grads) p.gate_bytes = round16((p.ranges + gate_grads) * n * 4);
+  return p;
+}
+
+template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS>
+static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan& plan)
+{
+  const int threads = (TEAM == 16 ? 16 : kWave * plan.shape.nw) * plan.teams;
+  const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(threads * 8 * sizeof(float)) : 0;
+  hipLaunchKernelGGL((rn_bwd_rows<T, TEAM, BRANCH_NORM, GATE, BIAS>), dim3(static_cast<unsigned>(plan.ranges)), dim3(threads), lds,
+                     st, a, plan.shape.nw);
+}
+
+template <typename T, int TEAM>
+static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan& plan, bool bias)
+{
+  const bool norm = a.branch_norm != kNormNone, gate = a.gate != nullptr;
+  if (norm) {
+    if (gate) bias ? rn_launch_bwd<T, TEAM, true, true, true>(st, a, plan) : rn_launch_bwd<T, TEAM, true, true, false>(st, a, plan);
+    else bias ? rn_launch_bwd<T, TEAM, true, false, true>(st, a, plan) : rn_launch_bwd<T, TEAM, true, false, false>(st, a, plan);
+  }
+  else {
+    if (gate) bias ? rn_launch_bwd<T, TEAM, false, true, true>(st, a, plan) : rn_launch_bwd<T, TEAM, false, true, false>(st, a, plan);
+    else bias ? rn_launch_bwd<T, TEAM, false, false, true>(st, a, plan) : rn_launch_bwd<T, TEAM, false, false, false>(st, a, plan);
+  }
 }
 
 template <typename T, int V, bool SUB>
@@ -178,10 +224,11 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   bool weight_grads = false;
   for (float* d : dweights) weight_grads = weight_grads || d;
   const RnBwdPlan plan = rn_bwd_plan(a.n, a.width, weight_grads, dgate ? num_gates : 0);
-  if (!workspace || workspace_bytes < plan.total() || !aligned16(workspace)) return LBN_ERR_WORKSPACE;
+  if (plan.total() && (!workspace || workspace_bytes < plan.total() || !aligned16(workspace))) return LBN_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<float*>(ws);
   a.cols_per_range = plan.cols_per_range;
+  a.dgate = dgate, a.ld_dgate = ld_dgate;
   float* weights = reinterpret_cast<float*>(ws + plan.sums_bytes);
   RnMergeArgs merge{};
   for (int q = 0; q < kGradGate; ++q) {
@@ -192,18 +239,26 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   merge.part[kGradGate] = a.part[kGradGate], merge.out[kGradGate] = dgate;
   merge.n = a.n, merge.ranges = plan.ranges, merge.ld_dgate = ld_dgate, merge.num_gates = dgate ? num_gates : 0;
   merge.cols_per_gate = a.cols_per_gate, merge.cols_per_range = plan.cols_per_range;
+  const int64_t items = kGradGate + merge.num_gates;
+  auto capped = [](int64_t blocks) { return static_cast<unsigned>(blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30)); };
+  const dim3 merge_grid(capped(ceil_div(a.n, kMergeLanes)), static_cast<unsigned>(items < 32768 ? items : 32768));
 
   hipStream_t st = as_stream(stream);
-  auto capped = [](int64_t blocks) { return static_cast<unsigned>(blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30)); };
-  hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(capped(a.width)), dim3(kRnLongThreads), 0, st, a);
-  if (weight_grads || dgate) {
-    hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(capped(ceil_div(a.n, 2048)), static_cast<unsigned>(plan.ranges)), dim3(256),
-                       0, st, a);
-    const int64_t items = kGradGate + merge.num_gates;
-    hipLaunchKernelGGL(rn_merge, dim3(capped(ceil_div(a.n, 256)), static_cast<unsigned>(items < 32768 ? items : 32768)),
-                       dim3(256), 0, st, merge);
+  if (plan.shape.v) {
+    const bool bias = dweights[kGradOutputBias] || dweights[kGradBranchBias] || (dgate && a.branch_bias);
+    if (plan.shape.sub) rn_launch_bwd<T, 16>(st, a, plan, bias);
+    else if (plan.shape.nw <= 8) rn_launch_bwd<T, 512>(st, a, plan, bias);
+    else rn_launch_bwd<T, 1024>(st, a, plan, bias);
   }
-  hipLaunchKernelGGL((rn_bwd_long_apply<T>), dim3(capped(ceil_div(a.n, 2048) * a.width)), dim3(256), 0, st, a);
+  else {
+    hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(capped(a.width)), dim3(kRnLongThreads), 0, st, a);
+    if (weight_grads || dgate)
+      hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(capped(ceil_div(a.n, 2048)), static_cast<unsigned>(plan.ranges)),
+                         dim3(256), 0, st, a);
+    hipLaunchKernelGGL((rn_bwd_long_apply<T>), dim3(capped(ceil_div(a.n, 2048) * a.width)), dim3(256), 0, st, a);
+  }
+  if (weight_grads || dgate)
+    hipLaunchKernelGGL(rn_merge, merge_grid, dim3(kMergeLanes * kMergeGroups), 0, st, merge);
   return launch_status();
 }
 

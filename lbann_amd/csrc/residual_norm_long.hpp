@@ -70,6 +70,8 @@ struct RnBwdArgs {
   DropArgs drop;
   // partial gradients of ranges of columns; part[q] null: not wanted
   float* part[kGrads];
+  float* dgate;           // written at once for a gate whose columns all lie in one range
+  int64_t ld_dgate;
   float* sums;            // long kernels: four means per column
   int64_t cols_per_range;
 };
@@ -374,7 +376,8 @@ rn_bwd_long_columns(RnBwdArgs<T> a)
     if (a.part[kGradGate]) {
       const int64_t gate = col / a.cols_per_gate;
       if (col + 1 == last || (col + 1) / a.cols_per_gate != gate) {
-        store8(a.part[kGradGate] + (range + gate) * a.n + k, valid, acc[kGradGate]);
+        const bool whole = first <= gate * a.cols_per_gate && (gate + 1) * a.cols_per_gate <= last;
+        store8((whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (range + gate) * a.n) + k, valid, acc[kGradGate]);
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
       }

@@ -54,18 +54,22 @@ __device__ __forceinline__ float lanes_sum(float v)
   return SUB ? row16_sum(v) : wave_sum(v);
 }
 
-// Merges over the waves of a team (one team per workgroup when nw > 1).
+// Merges over the waves of a team, through sixteen slots a team.  Every team of the workgroup makes
+// the same calls.
+constexpr int kMergeSlots = 4 * 16;  // teams of two waves or more: at most four
+
 struct TeamMerge {
-  float2 (*slots)[16];  // two buffers, zero behind wave nw
+  float2 (*slots)[kMergeSlots];  // two buffers, zero behind a team's wave nw
   int nw, wave, lane;
+  int base;             // the team's first slot
   float count;          // entries of the column that wave (lane % 16) owns
   int turn = 0;
 
   __device__ __forceinline__ float2 exchange(float a, float b)
   {
-    if (lane == 0) slots[turn][wave] = make_float2(a, b);
+    if (lane == 0) slots[turn][base + wave] = make_float2(a, b);
     __syncthreads();
-    const float2 r = slots[turn][lane & 15];
+    const float2 r = slots[turn][base + (lane & 15)];
     turn ^= 1;  // the other buffer's barrier separates two uses of this one
     return r;
   }
@@ -120,7 +124,7 @@ template <int V, bool SUB>
 struct Team {
   int index, per_block, t;
   float inv_n, inv_mine;  // 1 / entries of the column, of this wave
-  __device__ __forceinline__ Team(int nw, int n, float2 (*slots)[16], TeamMerge& merge)
+  __device__ __forceinline__ Team(int nw, int n, float2 (*slots)[kMergeSlots], TeamMerge& merge)
   {
     const int tid = threadIdx.x;
     const int lanes = SUB ? 16 : kWave * nw;
@@ -131,6 +135,7 @@ struct Team {
     merge.nw = nw;
     merge.lane = tid & (kWave - 1);
     merge.wave = SUB ? 0 : wave_index() - index * nw;
+    merge.base = 16 * index;
     auto entries_of = [&](int wave) {
       int c = 0;
 #pragma unroll
@@ -148,7 +153,8 @@ struct Team {
       inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f;
       merge.count = (merge.lane & 15) < nw ? static_cast<float>(entries_of(merge.lane & 15)) : 0.f;
       if (nw > 1) {
-        if (tid < 32) slots[tid >> 4][tid & 15] = make_float2(0.f, 0.f);
+        for (int i = tid; i < 2 * kMergeSlots; i += static_cast<int>(blockDim.x))
+          slots[i / kMergeSlots][i % kMergeSlots] = make_float2(0.f, 0.f);
         __syncthreads();
       }
     }
@@ -163,7 +169,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   constexpr bool kKeepWeights = V == 1 || SUB;  // of a thread's units, in registers from column to column
   constexpr bool kPrefetch = V == 1 || SUB;
   constexpr int WV = kKeepWeights ? V : 1;
-  __shared__ float2 slots[2][16];
+  __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
   const int n = static_cast<int>(a.n);
   const Team<V, SUB> team(nw, n, slots, merge);
@@ -278,6 +284,218 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   };
   if (n == 8 * V * (SUB ? 16 : kWave * nw)) walk(std::true_type{});
   else walk(std::false_type{});
+}
+
+// ------------------------------------------------------------------ backward
+// A workgroup takes a contiguous range of columns; its teams (of 16 lanes or nw waves, one unit a
+// thread) walk it with the next column's loads in flight and sum the gradients of weights and
+// gate in registers.  At the end of the range, and for several gates at the end of each gate's
+// columns, the teams' sums are merged through LDS and leave one partial row.
+// BRANCH_NORM, GATE, BIAS: what there is to accumulate (BIAS: of any norm).
+//
+// Entries that do not exist are loaded as zeros and have zero weights, so that they add nothing
+// to any sum and need no masks.
+//
+// TEAM: lanes of the largest team.  Up to 512 (256 registers a thread) the weights of a thread's unit stay in
+// registers beside its up to five sums; teams of up to 1024 (128 registers) read them again for
+// every column, from L2.
+template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS>
+__global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
+rn_bwd_rows(RnBwdArgs<T> a, int nw)
+{
+  using U = Unit<T>;
+  constexpr bool SUB = TEAM == 16;
+  constexpr bool kKeepWeights = TEAM <= 512;
+  extern __shared__ float merged[];  // blockDim x 8 floats if there are several teams
+  __shared__ float2 slots[2][kMergeSlots];
+  TeamMerge merge;
+  const int n = static_cast<int>(a.n);
+  const Team<1, SUB> team(nw, n, slots, merge);
+  const RowShare<1> share(team.t, SUB ? 16 : kWave * nw, n);
+  const int unit = share.unit[0], valid = share.valid[0], entry = 8 * unit;
+  const int teams = team.per_block;
+  const DropStream stream = drop_stream(a.drop);
+  const bool dropping = a.drop.threshold < 65536u;
+  const bool several_gates = GATE && a.cols_per_gate < a.width;
+  const bool output_norm = a.output_norm != kNormNone;
+  const bool read_branch = BRANCH_NORM || (GATE && a.branch);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * a.cols_per_range;
+  const int64_t last = imin64(first + a.cols_per_range, a.width);
+
+  auto weights = [&](const float* w, float fill, float (&out)[8]) {
+    load_weights8(w, entry, valid, fill, out);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = j < valid ? out[j] : 0.f;
+  };
+  float w2[8], w1[8], b1[8], gt[8];
+  const float* gate_row = a.gate;
+  auto load_output_weights = [&] { weights(a.output_scale, 1.f, w2); };
+  auto load_branch_weights = [&] {
+    if (BRANCH_NORM) weights(a.branch_scale, 1.f, w1);
+    if (BRANCH_NORM && GATE && BIAS) weights(a.branch_bias, 0.f, b1);
+  };
+  auto load_gate = [&] {
+    if (GATE) weights(gate_row, 1.f, gt);
+  };
+  if constexpr (kKeepWeights) {
+    load_output_weights();
+    load_branch_weights();
+    load_gate();
+  }
+
+  float dw2[8] = {}, db2[8] = {}, dw1[8] = {}, db1[8] = {}, dg[8] = {};
+  typename U::raw_t qy{}, qh{}, qs{}, qo{};
+  RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
+  auto issue = [&](int64_t col) {
+    if (output_norm) {
+      qy = U::load(a.dy + col * a.ld_dy + entry, valid);
+      qs = U::load(a.h + col * a.ld_h + entry, valid);
+    }
+    if (a.dh) qh = U::load(a.dh + col * a.ld_dh + entry, valid);
+    if (read_branch) qo = U::load(a.branch + col * a.ld_branch + entry, valid);
+    if (BRANCH_NORM || output_norm) {
+      const float* st = a.stats + col * a.ld_stats;
+      qstats = {st[0], st[1], st[2], st[3]};  // variances, for now
+    }
+  };
+  // The sums of all teams, written as one row.
+  auto flush = [&](float (&acc)[8], float* row) {
+    if (teams == 1) {
+      store8(row + entry, valid, acc);
+    }
+    else {
+      const int lanes = static_cast<int>(blockDim.x) / teams;
+      __syncthreads();  // the rows before this one have been read
+#pragma unroll
+      for (int j = 0; j < 8; ++j) merged[(team.index * lanes + team.t) * 8 + j] = acc[j];
+      __syncthreads();
+      for (int k = threadIdx.x; k < 8 * lanes && k < n; k += blockDim.x) {
+        float s = 0.f;
+        for (int i = 0; i < teams; ++i) s += merged[i * 8 * lanes + k];
+        row[k] = s;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  };
+
+  bool in_flight = false;
+  for (int64_t begin = first; begin < last;) {
+    int64_t end = last, gate = 0;
+    if (several_gates) {
+      gate = begin / a.cols_per_gate;
+      end = imin64(last, (gate + 1) * a.cols_per_gate);
+      gate_row = a.gate + gate * a.ld_gate;
+      if (kKeepWeights) load_gate();
+    }
+    const int64_t turns = (end - begin + teams - 1) / teams;
+    int64_t col = begin + team.index;
+    if (!in_flight && col < end) issue(col);
+    for (int64_t turn = 0; turn < turns; ++turn, col += teams) {
+      const bool active = col < end;
+      float e[8], f[8], x[8];
+      RnColumnStats s = qstats;
+      s.rstd1 = BRANCH_NORM ? rn_rstd(s.rstd1 + a.epsilon) : 1.f;
+      s.rstd2 = rn_rstd(s.rstd2 + a.epsilon);
+      float o[8];
+      U::widen(qy, f);
+      U::widen(qs, x);
+      U::widen(qh, e);
+      U::widen(qo, o);
+      // a single team carries the next column over the end of a gate's columns
+      const int64_t next = col + teams;
+      in_flight = teams == 1 && next < last;
+      if (in_flight || next < end) issue(next);
+
+      if (output_norm) {
+        float sp = 0.f, spx = 0.f;
+        if constexpr (!kKeepWeights) load_output_weights();
+        if (active) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[j] = (x[j] - s.mean2) * s.rstd2;
+            dw2[j] = __builtin_fmaf(f[j], x[j], dw2[j]);
+            if (BIAS) db2[j] += f[j];
+            f[j] *= w2[j];
+            sp += f[j];
+            spx = __builtin_fmaf(f[j], x[j], spx);
+          }
+          sp = lanes_sum<SUB>(sp);
+          spx = lanes_sum<SUB>(spx);
+        }
+        if (!SUB && nw > 1) merge.sum2(sp, spx);
+        sp = a.output_norm == kNormLayer ? sp * team.inv_n : 0.f;
+        spx *= team.inv_n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = __builtin_fmaf(s.rstd2, f[j] - sp - x[j] * spx, e[j]);
+      }
+      if (active && a.dresidual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = a.residual_mult * e[j];
+        store8(a.dresidual + col * a.ld_dresidual + entry, valid, f);
+      }
+      // e becomes du; o the normalised branch
+      if constexpr (!kKeepWeights) {
+        load_branch_weights();
+        load_gate();
+      }
+      float keep[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) keep[j] = 1.f;
+      if (dropping) {
+        uint32_t w[4];
+        drop_words(a.drop, stream, unit, static_cast<uint32_t>(col), w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) keep[j] = drop_kept(w, j, a.drop.threshold) ? a.drop.inverse_keep : 0.f;
+      }
+      if (BRANCH_NORM) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = (o[j] - s.mean1) * s.rstd1;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = keep[j] != 0.f ? a.branch_mult * e[j] * keep[j] : 0.f;
+        if (GATE) {
+          if (active && read_branch) {
+            const float u = BRANCH_NORM ? (BIAS ? __builtin_fmaf(o[j], w1[j], b1[j]) : o[j] * w1[j]) : o[j];
+            dg[j] += keep[j] != 0.f ? e[j] * u : 0.f;
+          }
+          e[j] *= gt[j];
+          if (dropping) e[j] = keep[j] != 0.f ? e[j] : 0.f;
+        }
+      }
+      if (BRANCH_NORM) {
+        float sp = 0.f, spu = 0.f;
+        if (active) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            dw1[j] = __builtin_fmaf(e[j], o[j], dw1[j]);
+            if (BIAS) db1[j] += e[j];
+            e[j] *= w1[j];
+            sp += e[j];
+            spu = __builtin_fmaf(e[j], o[j], spu);
+          }
+          sp = lanes_sum<SUB>(sp);
+          spu = lanes_sum<SUB>(spu);
+        }
+        if (!SUB && nw > 1) merge.sum2(sp, spu);
+        sp = a.branch_norm == kNormLayer ? sp * team.inv_n : 0.f;
+        spu *= team.inv_n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = s.rstd1 * (e[j] - sp - o[j] * spu);
+      }
+      if (active) store8(a.dbranch + col * a.ld_dbranch + entry, valid, e);
+    }
+    if (GATE && a.part[kGradGate] && (several_gates || end == last)) {
+      const bool whole = begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate;
+      flush(dg, whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (blockIdx.x + gate) * a.n);
+    }
+    begin = end;
+  }
+  if (a.part[kGradOutputScale]) flush(dw2, a.part[kGradOutputScale] + blockIdx.x * a.n);
+  if (BIAS && a.part[kGradOutputBias]) flush(db2, a.part[kGradOutputBias] + blockIdx.x * a.n);
+  if (BRANCH_NORM && a.part[kGradBranchScale]) flush(dw1, a.part[kGradBranchScale] + blockIdx.x * a.n);
+  if (BRANCH_NORM && BIAS && a.part[kGradBranchBias]) flush(db1, a.part[kGradBranchBias] + blockIdx.x * a.n);
 }
 
 }  // namespace lbn
