@@ -782,28 +782,52 @@ def softmax_cross_entropy_backward(softmax, cross_entropy, dloss, want_dtruth=Fa
 
 
 _SUFFIX = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}
+_ENTRIES = {}
 
 
-def _suffix_of(m):
-    try:
-        return _SUFFIX[m.dtype]
-    except KeyError:
-        raise TypeError(f"storage is fp32, fp16 or bfloat16, not {m.dtype}") from None
+def _entry(name, dtype):
+    """The entry point of `name` for a storage type (a decoding step makes these calls in a row
+    on a few microseconds' work each, so nothing here is looked up twice)."""
+    f = _ENTRIES.get((name, dtype))
+    if f is None:
+        if dtype not in _SUFFIX:
+            raise TypeError(f"storage is fp32, fp16 or bfloat16, not {dtype}")
+        full = f"{name}_{_SUFFIX[dtype]}"
+        entry = getattr(capi.lib(), full)
+
+        def f(*args):
+            status = entry(*args)
+            if status:
+                raise LbnError(full, status, capi.lib().lbn_status_string(status).decode())
+        _ENTRIES[name, dtype] = f
+    return f
 
 
 def _same_kind(like, height, width, **matrices):
     """Every given matrix has the shape, the storage type and the device of `like`."""
+    t = like.tensor
     for name, m in matrices.items():
-        if m is not None and ((m.height, m.width) != (height, width) or m.dtype != like.dtype
-                              or m.tensor.device != like.tensor.device):
+        if m is not None and (m.height != height or m.width != width or m.tensor.dtype != t.dtype
+                              or m.tensor.get_device() != t.get_device()):
             raise ValueError(f"{name} is {m.height} x {m.width} {m.dtype} on {m.tensor.device}; expected "
-                             f"{height} x {width} {like.dtype} on {like.tensor.device}")
+                             f"{height} x {width} {t.dtype} on {t.device}")
 
 
-def _on_current_device(m):
-    """Kernels go to the current stream of the current device: refuse matrices of another one."""
-    if m.tensor.device.type != "cuda" or m.tensor.device.index != torch.cuda.current_device():
+def _stream_for(m):
+    """The current stream, as an address.  Kernels go to the current device: refuse matrices of
+    another one."""
+    index = m.tensor.get_device()  # negative for host memory
+    if index < 0 or index != torch.cuda.current_device():
         raise ValueError(f"matrix on {m.tensor.device}; the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _matrix_beside(like, height, width, dtype=None):
+    """An uninitialised matrix on the device of `like`, of its storage type unless another is given."""
+    m = DeviceMatrix.__new__(DeviceMatrix)
+    m.height, m.width, m.ldim = height, width, max(height, 1)
+    m.tensor = like.tensor.new_empty((max(width, 1), m.ldim), dtype=dtype)
+    return m
 
 
 def _pointer(t):
@@ -820,7 +844,7 @@ def _device_values(t, n, dtype, what, like):
     if t is None:
         return None
     t = getattr(t, "tensor", t)
-    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (n > 1 and t.stride(0) != 1) or t.device != like.tensor.device:
+    if t.dtype != dtype or t.dim() != 1 or t.numel() < n or (n > 1 and t.stride(0) != 1) or t.get_device() != like.tensor.get_device():
         raise ValueError(f"{what}: expected {n} contiguous {dtype} values on {like.tensor.device}")
     return t.data_ptr()
 
@@ -869,17 +893,23 @@ class dropout_layer(_Layer, _Dropout):
         self._start(training, offset)
         return super().forward(x, in_place)
 
-    def _call(self, direction, x, y):
+    def bind_forward(self, x, in_place=False):
+        self.prev_activations = x
+        self.activations = x if in_place else _matrix_beside(x, x.height, x.width)
+
+    def bind_backward(self, dy, in_place=False):
+        self.prev_error_signals = dy
+        self.error_signals = dy if in_place else _matrix_beside(dy, dy.height, dy.width)
+
+    def _run(self, name, x, y):
         _same_kind(x, x.height, x.width, output=y)
-        _on_current_device(x)
-        return (f"lbn_dropout_{direction}_{_suffix_of(x)}",
-                (_stream(), x.height, x.width, *self._drop_args(x), *_buffer(x), *_buffer(y)))
+        _entry(name, x.tensor.dtype)(_stream_for(x), x.height, x.width, *self._drop_args(x), *_buffer(x), *_buffer(y))
 
-    def fp_call(self):
-        return self._call("fwd", self.prev_activations, self.activations)
+    def fp_compute(self):
+        self._run("lbn_dropout_fwd", self.prev_activations, self.activations)
 
-    def bp_call(self):
-        return self._call("bwd", self.prev_error_signals, self.error_signals)
+    def bp_compute(self):
+        self._run("lbn_dropout_bwd", self.prev_error_signals, self.error_signals)
 
 
 class residual_norm_layer(_Dropout):
@@ -930,39 +960,34 @@ class residual_norm_layer(_Dropout):
         for name in self.weights:
             setattr(self, f"m_{name}_gradient", None)
 
-    def _new(self, like, width, height=None, dtype=None):
-        return DeviceMatrix(self.size if height is None else height, width, dtype=dtype or like.dtype,
-                            device=like.tensor.device)
-
     def _check_gate(self, gate, like):
         if gate is None:
             return
-        if gate.height != self.size or gate.width < 1 or like.width % gate.width or gate.dtype != torch.float32 \
-                or gate.tensor.device != like.tensor.device:
+        if gate.height != self.size or gate.width < 1 or like.width % gate.width or gate.tensor.dtype != torch.float32 \
+                or gate.tensor.get_device() != like.tensor.get_device():
             raise ValueError(f"gate is {gate.height} x {gate.width} {gate.dtype}; expected {self.size} rows of fp32 on "
                              f"{like.tensor.device} and a number of columns that divides {like.width}")
 
     def forward(self, branch, residual=None, gate=None, training=True, offset=None, in_place=False):
         """in_place: the new stream overwrites `residual` and y overwrites `branch` (inference: backward
         needs what they held).  training=False: no dropout, no statistics."""
-        _same_kind(branch, self.size, branch.width, branch=branch, residual=residual)
-        _on_current_device(branch)
+        n, w, kinds, wt = self.size, branch.width, self._kinds, self.weights
+        _same_kind(branch, n, w, branch=branch, residual=residual)
+        stream = _stream_for(branch)
         self._check_gate(gate, branch)
         self._start(training, offset)
-        w = branch.width
         self.branch, self.gate, self.m_has_residual = branch, gate, residual is not None
-        stream_out = residual if in_place and residual is not None else self._new(branch, w)
+        h = residual if in_place and residual is not None else _matrix_beside(branch, n, w)
         y = None
-        if self._kinds[1]:
-            y = branch if in_place else self._new(branch, w)
-        self.m_statistics = self._new(branch, w, 4, torch.float32) if training else None
-        wt = self.weights
-        call(f"lbn_residual_norm_fwd_{_suffix_of(branch)}", _stream(), self.size, w, *self._kinds, self.m_epsilon,
-             self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch), *_buffer(residual), *_buffer(gate),
-             gate.width if gate is not None else 0, _pointer(wt["branch_scale"]), _pointer(wt["branch_bias"]),
-             _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch), *_buffer(stream_out),
-             *_buffer(y), *_buffer(self.m_statistics))
-        self.h = self.residual = stream_out
+        if kinds[1]:
+            y = branch if in_place else _matrix_beside(branch, n, w)
+        self.m_statistics = _matrix_beside(branch, 4, w, torch.float32) if training else None
+        _entry("lbn_residual_norm_fwd", branch.tensor.dtype)(
+            stream, n, w, *kinds, self.m_epsilon, self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch),
+            *_buffer(residual), *_buffer(gate), 0 if gate is None else gate.width, _pointer(wt["branch_scale"]),
+            _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch),
+            *_buffer(h), *_buffer(y), *_buffer(self.m_statistics))
+        self.h = self.residual = h
         self.activations = y
         return y
 
@@ -980,30 +1005,29 @@ class residual_norm_layer(_Dropout):
             raise ValueError("backward takes dy exactly if there is an output norm, and dresidual if there is none")
         if self.m_statistics is None:
             raise ValueError("backward needs a training-mode forward (or bind_saved) first")
-        w = like.width
-        _same_kind(like, self.size, w, dy=dy, dresidual=dresidual, branch=self.branch, h=self.h)
-        if (self.m_statistics.height, self.m_statistics.width, self.m_statistics.dtype) != (4, w, torch.float32):
+        n, w, kinds, wt, gate = self.size, like.width, self._kinds, self.weights, self.gate
+        _same_kind(like, n, w, dy=dy, dresidual=dresidual, branch=self.branch, h=self.h)
+        st = self.m_statistics
+        if st.height != 4 or st.width != w or st.tensor.dtype != torch.float32 or st.tensor.get_device() != like.tensor.get_device():
             raise ValueError("the statistics are a (4 x width) fp32 matrix")
-        _on_current_device(like)
-        dbranch = self._new(like, w)
-        dres = self._new(like, w) if self.m_has_residual else None
-        wt, kinds = self.weights, self._kinds
-        for name, t in wt.items():
-            setattr(self, f"m_{name}_gradient", None if t is None else _Vector(self.size, like.tensor.device))
-        gate = self.gate
-        self.m_gate_gradient = None if gate is None else DeviceMatrix(self.size, gate.width, device=like.tensor.device)
-        grads = [getattr(self, f"m_{name}_gradient") for name in ("branch_scale", "branch_bias", "output_scale", "output_bias")]
-        gates = gate.width if gate is not None else 0
-        need = capi.lib().lbn_residual_norm_bwd_workspace_bytes(
-            self.size, w, int(any(g is not None for g in grads)), gates, like.tensor.element_size())
+        stream = _stream_for(like)
+        dbranch = _matrix_beside(like, n, w)
+        dres = _matrix_beside(like, n, w) if self.m_has_residual else None
+        grads = []
+        for name in ("branch_scale", "branch_bias", "output_scale", "output_bias"):
+            g = None if wt[name] is None else _Vector(n, like.tensor.device)
+            setattr(self, f"m_{name}_gradient", g)
+            grads.append(None if g is None else g.tensor.data_ptr())
+        gates = 0 if gate is None else gate.width
+        self.m_gate_gradient = dgate = None if gate is None else _matrix_beside(like, n, gates, torch.float32)
+        need = capi.lib().lbn_residual_norm_bwd_workspace_bytes(n, w, int(any(grads)), gates, like.tensor.element_size())
         # scratch of this call alone: nothing that another stream or a recorded graph could share
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=like.tensor.device)
-        call(f"lbn_residual_norm_bwd_{_suffix_of(like)}", _stream(), self.size, w, *kinds, self.m_epsilon,
-             self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(self.branch),
-             *(_buffer(self.h) if kinds[1] else (None, 0)), *_buffer(gate), gates, _pointer(wt["branch_scale"]),
-             _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), *self._drop_args(like), *_buffer(self.m_statistics),
-             *_buffer(dy), *_buffer(dresidual), *_buffer(dbranch), *_buffer(dres), *_buffer(self.m_gate_gradient),
-             *(_pointer(None if g is None else g.tensor) for g in grads), ws.data_ptr(), need)
+        ws = like.tensor.new_empty((need,), dtype=torch.uint8) if need else None
+        _entry("lbn_residual_norm_bwd", like.tensor.dtype)(
+            stream, n, w, *kinds, self.m_epsilon, self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(self.branch),
+            *(_buffer(self.h) if kinds[1] else (None, 0)), *_buffer(gate), gates, _pointer(wt["branch_scale"]),
+            _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), *self._drop_args(like), *_buffer(st), *_buffer(dy),
+            *_buffer(dresidual), *_buffer(dbranch), *_buffer(dres), *_buffer(dgate), *grads, _pointer(ws), need)
         return dbranch, dres
 
 
@@ -1021,7 +1045,7 @@ class logits_adjust_layer:
     def _matrix(m, width, dtype, what, like, height=None):
         if m is None:
             return None, 0, 0
-        if m.dtype != dtype or m.tensor.device != like.tensor.device or (width is not None and m.width != width) \
+        if m.tensor.dtype != dtype or m.tensor.get_device() != like.tensor.get_device() or (width is not None and m.width != width) \
                 or (height is not None and m.height != height):
             raise ValueError(f"{what} is {m.height} x {m.width} {m.dtype} on {m.tensor.device}")
         return m.tensor.data_ptr(), m.ldim, m.height
@@ -1034,8 +1058,8 @@ class logits_adjust_layer:
         grammars) int32 words, mask_index an int32 vector.  Everything but x is optional."""
         w = x.width
         _same_kind(x, self.vocabulary, w, logits=x)
-        _on_current_device(x)
-        y = x if in_place else DeviceMatrix(self.vocabulary, w, dtype=x.dtype, device=x.tensor.device)
+        stream = _stream_for(x)
+        y = x if in_place else _matrix_beside(x, self.vocabulary, w)
         if (bias_tokens is None) != (bias_values is None):
             raise ValueError("bias_tokens and bias_values go together")
         words = (self.vocabulary + 31) // 32
@@ -1043,13 +1067,14 @@ class logits_adjust_layer:
         bt, ld_bt, biases = self._matrix(bias_tokens, w, torch.int32, "bias_tokens", x)
         bv, ld_bv, _ = self._matrix(bias_values, w, torch.float32, "bias_values", x, biases or None)
         mk, ld_mk, _ = self._matrix(mask, None, torch.int32, "mask", x, words)
-        call(f"lbn_logits_adjust_{_suffix_of(x)}", _stream(), self.vocabulary, w, *_buffer(x), *_buffer(y), tok, ld_tok,
-             max_tokens, _device_values(lengths, w, torch.int32, "lengths", x),
-             _device_values(prompt_lengths, w, torch.int32, "prompt_lengths", x),
-             _device_values(repetition, w, torch.float32, "repetition", x),
-             _device_values(presence, w, torch.float32, "presence", x),
-             _device_values(frequency, w, torch.float32, "frequency", x), bt, ld_bt, bv, ld_bv, biases, mk, ld_mk,
-             mask.width if mask is not None else 0, _device_values(mask_index, w, torch.int32, "mask_index", x))
+        _entry("lbn_logits_adjust", x.tensor.dtype)(
+            stream, self.vocabulary, w, *_buffer(x), *_buffer(y), tok, ld_tok, max_tokens,
+            _device_values(lengths, w, torch.int32, "lengths", x),
+            _device_values(prompt_lengths, w, torch.int32, "prompt_lengths", x),
+            _device_values(repetition, w, torch.float32, "repetition", x),
+            _device_values(presence, w, torch.float32, "presence", x),
+            _device_values(frequency, w, torch.float32, "frequency", x), bt, ld_bt, bv, ld_bv, biases, mk, ld_mk,
+            0 if mask is None else mask.width, _device_values(mask_index, w, torch.int32, "mask_index", x))
         self.activations = y
         return y
 
