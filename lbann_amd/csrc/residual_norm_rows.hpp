@@ -15,16 +15,57 @@
 
 namespace lbn {
 
+// Eight entries as they are stored.  A column whose length is no multiple of eight ends in a partial
+// unit: it is read as the last eight entries of the column and moved down by `shift` entries when
+// it is used, which leaves zeros where nothing is.  So every load is whole, waits for nothing and stays inside the
+// column (columns have at least eight entries here), and only the wave with the partial unit moves
+// anything.
 template <typename T>
 struct Unit {
   typedef T raw_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
-  static __device__ __forceinline__ raw_t load(const T* p, int valid)
+  static __device__ __forceinline__ raw_t load(const T* p) { return *reinterpret_cast<const raw_t*>(p); }
+  static __device__ __forceinline__ raw_t moved(const raw_t& r, int shift)
   {
-    if (valid == 8) return *reinterpret_cast<const raw_t*>(p);
-    raw_t r;
+    constexpr int W = 2 * static_cast<int>(sizeof(T));  // words of a unit
+    uint32_t d[W + 4];
+    __builtin_memcpy(d, &r, 4 * W);
+    if constexpr (sizeof(T) == 2) {
+      if (shift & 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = j < valid ? p[j] : static_cast<T>(0.f);
-    return r;
+        for (int i = 0; i < W; ++i) d[i] = d[i] >> 16 | (i + 1 < W ? d[i + 1] << 16 : 0u);
+      }
+      shift >>= 1;
+    }
+#pragma unroll
+    for (int by = 1; by < W; by *= 2) {
+      if (shift & by) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) d[i] = i + by < W ? d[i + by] : 0u;
+      }
+    }
+    if (shift & W) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) d[i] = 0u;
+    }
+    raw_t out;
+    __builtin_memcpy(&out, d, 4 * W);
+    return out;
+  }
+  // EVEN: the length is a multiple of eight, a unit exists (shift 0) or does not (8).
+  template <bool EVEN>
+  static __device__ __forceinline__ void widen(raw_t r, int shift, float (&v)[8])
+  {
+    if constexpr (EVEN) {
+      uint32_t d[sizeof(raw_t) / 4];
+      __builtin_memcpy(d, &r, sizeof(d));
+#pragma unroll
+      for (uint32_t& w : d) w = shift ? 0u : w;
+      __builtin_memcpy(&r, d, sizeof(d));
+    }
+    else if (shift) {
+      r = moved(r, shift);
+    }
+    widen(r, v);
   }
   static __device__ __forceinline__ void widen(const raw_t& r, float (&v)[8])
   {
@@ -33,10 +74,31 @@ struct Unit {
   }
 };
 
-// Which entries of its column a thread owns: unit(i) = t + i * lanes, valid[i] of its entries exist.
-template <int V>
+// Eight entries in the storage type: the whole unit, or its first `valid` ones in up to three pieces.
+template <bool EVEN, typename T>
+__device__ __forceinline__ void store_unit(T* p, int valid, const float (&v)[8])
+{
+  if (valid == 8) {
+    store8(p, 8, v);
+  }
+  else if constexpr (!EVEN) {
+    T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = static_cast<T>(v[j]);
+    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    typedef T two_t __attribute__((ext_vector_type(2), aligned(sizeof(T))));
+    const bool four = valid & 4, two = valid & 2;
+    if (four) *reinterpret_cast<four_t*>(p) = four_t{t[0], t[1], t[2], t[3]};
+    T a = four ? t[4] : t[0], b = four ? t[5] : t[1], c = four ? t[6] : t[2];
+    if (two) *reinterpret_cast<two_t*>(p + (valid & 4)) = two_t{a, b};
+    if (valid & 1) p[valid & 6] = two ? c : a;
+  }
+}
+
+// Which entries of its column a thread owns: unit(i) = t + i * lanes, of which valid[i] entries exist.
+template <int V, bool EVEN>
 struct RowShare {
-  int unit[V], valid[V];
+  int unit[V], valid[V], at[V], shift[V];  // where the unit is read, and how far it is moved then
   __device__ __forceinline__ RowShare(int t, int lanes, int n)
   {
 #pragma unroll
@@ -44,6 +106,19 @@ struct RowShare {
       unit[i] = t + i * lanes;
       const int left = n - 8 * unit[i];
       valid[i] = left < 0 ? 0 : (left > 8 ? 8 : left);
+      at[i] = left < 8 ? n - 8 : 8 * unit[i];
+      shift[i] = 8 - valid[i];
+    }
+  }
+  // The thread's entries of a weight vector (null: `fill`); 0 where nothing exists.
+  __device__ __forceinline__ void weights(const float* w, int i, float fill, float (&out)[8]) const
+  {
+    if (w) {
+      Unit<float>::template widen<EVEN>(Unit<float>::load(w + at[i]), shift[i], out);
+    }
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out[j] = j < valid[i] ? fill : 0.f;
     }
   }
 };
@@ -81,9 +156,9 @@ struct TeamMerge {
   }
 };
 
-// Mean and variance of a column from registers.  Entries that do not exist do not count.
-template <int V, bool SUB, bool FULL>
-__device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowShare<V>& share, int kind, float inv_n,
+// Mean and variance of a column from registers.  Entries that do not exist are zeros and do not count.
+template <int V, bool SUB, bool FULL, bool EVEN>
+__device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowShare<V, EVEN>& share, int kind, float inv_n,
                                             float inv_mine, TeamMerge& merge, float& mean, float& var)
 {
   float part_mean = 0.f;
@@ -92,7 +167,7 @@ __device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowSha
 #pragma unroll
     for (int i = 0; i < V; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += FULL || j < share.valid[i] ? x[i][j] : 0.f;
+      for (int j = 0; j < 8; ++j) s += x[i][j];
     part_mean = lanes_sum<SUB>(s) * inv_mine;
   }
   float q = 0.f;
@@ -100,7 +175,7 @@ __device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowSha
   for (int i = 0; i < V; ++i)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float d = FULL || j < share.valid[i] ? x[i][j] - part_mean : 0.f;
+      const float d = FULL || (EVEN ? share.valid[i] != 0 : j < share.valid[i]) ? x[i][j] - part_mean : 0.f;
       q = __builtin_fmaf(d, d, q);
     }
   q = lanes_sum<SUB>(q);
@@ -161,7 +236,7 @@ struct Team {
   }
 };
 
-template <typename T, int V, bool SUB>
+template <typename T, int V, bool SUB, bool EVEN>
 __global__ void __launch_bounds__(SUB ? 256 : 1024)
 rn_fwd_rows(RnFwdArgs<T> a, int nw)
 {
@@ -173,15 +248,13 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   TeamMerge merge;
   const int n = static_cast<int>(a.n);
   const Team<V, SUB> team(nw, n, slots, merge);
-  const RowShare<V> share(team.t, SUB ? 16 : kWave * nw, n);
+  const RowShare<V, EVEN> share(team.t, SUB ? 16 : kWave * nw, n);
   const DropStream stream = drop_stream(a.drop);
   const bool dropping = a.drop.threshold < 65536u;
   const bool one_gate = a.gate && a.cols_per_gate == a.width;
 
   auto gate_of = [&](int64_t col) { return a.gate ? a.gate + col / a.cols_per_gate * a.ld_gate : nullptr; };
-  auto weights = [&](const float* w, int i, float fill, float (&out)[8]) {
-    load_weights8(w, 8 * share.unit[i], share.valid[i], fill, out);
-  };
+  auto weights = [&](const float* w, int i, float fill, float (&out)[8]) { share.weights(w, i, fill, out); };
   float w1[WV][8], b1[WV][8], w2[WV][8], b2[WV][8], gt[WV][8];
   if constexpr (kKeepWeights) {
 #pragma unroll
@@ -198,11 +271,11 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   auto issue = [&](int64_t col) {
     const T* o = a.branch + col * a.ld_branch;
 #pragma unroll
-    for (int i = 0; i < V; ++i) qo[i] = U::load(o + 8 * share.unit[i], share.valid[i]);
+    for (int i = 0; i < V; ++i) qo[i] = U::load(o + share.at[i]);
     if (a.residual) {
       const T* r = a.residual + col * a.ld_residual;
 #pragma unroll
-      for (int i = 0; i < V; ++i) qr[i] = U::load(r + 8 * share.unit[i], share.valid[i]);
+      for (int i = 0; i < V; ++i) qr[i] = U::load(r + share.at[i]);
     }
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * team.per_block;
@@ -216,10 +289,16 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
       if (!kPrefetch) issue(col);
       float x[V][8], r[V][8];
 #pragma unroll
-      for (int i = 0; i < V; ++i) U::widen(qo[i], x[i]);
+      for (int i = 0; i < V; ++i) {
+        if constexpr (kFull) U::widen(qo[i], x[i]);
+        else U::template widen<EVEN>(qo[i], share.shift[i], x[i]);
+      }
       if (a.residual) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) U::widen(qr[i], r[i]);
+        for (int i = 0; i < V; ++i) {
+        if constexpr (kFull) U::widen(qr[i], r[i]);
+        else U::template widen<EVEN>(qr[i], share.shift[i], r[i]);
+      }
       }
       if (kPrefetch && col + step < a.width) issue(col + step);
       if (a.gate && !one_gate && kKeepWeights) {
@@ -228,7 +307,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
       }
       float mean1 = 0.f, var1 = 1.f, mean2 = 0.f, var2 = 1.f;
       if (a.branch_norm != kNormNone) {
-        row_moments<V, SUB, kFull>(x, share, a.branch_norm, team.inv_n, team.inv_mine, merge, mean1, var1);
+        row_moments<V, SUB, kFull, EVEN>(x, share, a.branch_norm, team.inv_n, team.inv_mine, merge, mean1, var1);
         const float rstd = rn_rstd(var1 + a.epsilon);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -258,10 +337,10 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
           x[i][j] *= a.branch_mult * gt[kw ? i : 0][j];
           if (a.residual) x[i][j] = __builtin_fmaf(a.residual_mult, r[i][j], x[i][j]);
         }
-        if (a.h) store8(a.h + col * a.ld_h + 8 * share.unit[i], share.valid[i], x[i]);
+        if (a.h) store_unit<EVEN>(a.h + col * a.ld_h + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
       }
       if (a.output_norm != kNormNone) {
-        row_moments<V, SUB, kFull>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
+        row_moments<V, SUB, kFull, EVEN>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
         const float rstd = rn_rstd(var2 + a.epsilon);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -273,7 +352,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             x[i][j] = __builtin_fmaf((x[i][j] - mean2) * rstd, w2[kw ? i : 0][j], b2[kw ? i : 0][j]);
-          store8(a.y + col * a.ld_y + 8 * share.unit[i], share.valid[i], x[i]);
+          store_unit<EVEN>(a.y + col * a.ld_y + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
         }
       }
       if (a.stats && team.t == 0) {
@@ -282,7 +361,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
       }
     }
   };
-  if (n == 8 * V * (SUB ? 16 : kWave * nw)) walk(std::true_type{});
+  if (EVEN && n == 8 * V * (SUB ? 16 : kWave * nw)) walk(std::integral_constant<bool, EVEN>{});
   else walk(std::false_type{});
 }
 
@@ -291,7 +370,8 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
 // thread) walk it with the next column's loads in flight and sum the gradients of weights and
 // gate in registers.  At the end of the range, and for several gates at the end of each gate's
 // columns, the teams' sums are merged through LDS and leave one partial row.
-// BRANCH_NORM, GATE, BIAS: what there is to accumulate (BIAS: of any norm).
+// BRANCH_NORM, GATE, BIAS: what there is to accumulate (BIAS: of any norm); GATE and BIAS may be
+// set where there is none.  EVEN: the length is a multiple of eight.
 //
 // Entries that do not exist are loaded as zeros and have zero weights, so that they add nothing
 // to any sum and need no masks.
@@ -299,7 +379,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
 // TEAM: lanes of the largest team.  Up to 512 (256 registers a thread) the weights of a thread's unit stay in
 // registers beside its up to five sums; teams of up to 1024 (128 registers) read them again for
 // every column, from L2.
-template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS>
+template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN>
 __global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
 rn_bwd_rows(RnBwdArgs<T> a, int nw)
 {
@@ -311,8 +391,8 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   TeamMerge merge;
   const int n = static_cast<int>(a.n);
   const Team<1, SUB> team(nw, n, slots, merge);
-  const RowShare<1> share(team.t, SUB ? 16 : kWave * nw, n);
-  const int unit = share.unit[0], valid = share.valid[0], entry = 8 * unit;
+  const RowShare<1, EVEN> share(team.t, SUB ? 16 : kWave * nw, n);
+  const int unit = share.unit[0], valid = share.valid[0], entry = 8 * unit, at = share.at[0], shift = share.shift[0];
   const int teams = team.per_block;
   const DropStream stream = drop_stream(a.drop);
   const bool dropping = a.drop.threshold < 65536u;
@@ -322,11 +402,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   const int64_t first = static_cast<int64_t>(blockIdx.x) * a.cols_per_range;
   const int64_t last = imin64(first + a.cols_per_range, a.width);
 
-  auto weights = [&](const float* w, float fill, float (&out)[8]) {
-    load_weights8(w, entry, valid, fill, out);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = j < valid ? out[j] : 0.f;
-  };
+  auto weights = [&](const float* w, float fill, float (&out)[8]) { share.weights(w, 0, fill, out); };
   float w2[8], w1[8], b1[8], gt[8];
   const float* gate_row = a.gate;
   auto load_output_weights = [&] { weights(a.output_scale, 1.f, w2); };
@@ -348,11 +424,11 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
   auto issue = [&](int64_t col) {
     if (output_norm) {
-      qy = U::load(a.dy + col * a.ld_dy + entry, valid);
-      qs = U::load(a.h + col * a.ld_h + entry, valid);
+      qy = U::load(a.dy + col * a.ld_dy + at);
+      qs = U::load(a.h + col * a.ld_h + at);
     }
-    if (a.dh) qh = U::load(a.dh + col * a.ld_dh + entry, valid);
-    if (read_branch) qo = U::load(a.branch + col * a.ld_branch + entry, valid);
+    if (a.dh) qh = U::load(a.dh + col * a.ld_dh + at);
+    if (read_branch) qo = U::load(a.branch + col * a.ld_branch + at);
     if (BRANCH_NORM || output_norm) {
       const float* st = a.stats + col * a.ld_stats;
       qstats = {st[0], st[1], st[2], st[3]};  // variances, for now
@@ -361,7 +437,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   // The sums of all teams, written as one row.
   auto flush = [&](float (&acc)[8], float* row) {
     if (teams == 1) {
-      store8(row + entry, valid, acc);
+      store_unit<EVEN>(row + entry, valid, acc);
     }
     else {
       const int lanes = static_cast<int>(blockDim.x) / teams;
@@ -398,10 +474,10 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       s.rstd1 = BRANCH_NORM ? rn_rstd(s.rstd1 + a.epsilon) : 1.f;
       s.rstd2 = rn_rstd(s.rstd2 + a.epsilon);
       float o[8];
-      U::widen(qy, f);
-      U::widen(qs, x);
-      U::widen(qh, e);
-      U::widen(qo, o);
+      U::template widen<EVEN>(qy, shift, f);
+      U::template widen<EVEN>(qs, shift, x);
+      U::template widen<EVEN>(qh, shift, e);
+      U::template widen<EVEN>(qo, shift, o);
       // a single team carries the next column over the end of a gate's columns
       const int64_t next = col + teams;
       in_flight = teams == 1 && next < last;
@@ -432,7 +508,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       if (active && a.dresidual) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = a.residual_mult * e[j];
-        store8(a.dresidual + col * a.ld_dresidual + entry, valid, f);
+        store_unit<EVEN>(a.dresidual + col * a.ld_dresidual + entry, valid, f);
       }
       // e becomes du; o the normalised branch
       if constexpr (!kKeepWeights) {
@@ -484,7 +560,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = s.rstd1 * (e[j] - sp - o[j] * spu);
       }
-      if (active) store8(a.dbranch + col * a.ld_dbranch + entry, valid, e);
+      if (active) store_unit<EVEN>(a.dbranch + col * a.ld_dbranch + entry, valid, e);
     }
     if (GATE && a.part[kGradGate] && (several_gates || end == last)) {
       const bool whole = begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate;
