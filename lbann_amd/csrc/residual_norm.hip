@@ -149,7 +149,7 @@ template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVE
 static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan& plan)
 {
   const int threads = (TEAM == 16 ? 16 : kWave * plan.shape.nw) * plan.teams;
-  const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(threads * 8 * sizeof(float)) : 0;
+  const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(kMergeRows * threads * 8 * sizeof(float)) : 0;
   hipLaunchKernelGGL((rn_bwd_rows<T, TEAM, BRANCH_NORM, GATE, BIAS, EVEN>), dim3(static_cast<unsigned>(plan.ranges)), dim3(threads),
                      lds, st, a, plan.shape.nw);
 }
@@ -255,7 +255,7 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   float* weights = reinterpret_cast<float*>(ws + plan.sums_bytes);
   RnMergeArgs merge{};
   for (int q = 0; q < kGradGate; ++q) {
-    a.part[q] = dweights[q] ? weights + q * plan.ranges * a.n : nullptr;
+    a.part[q] = !dweights[q] ? nullptr : plan.ranges == 1 ? dweights[q] : weights + q * plan.ranges * a.n;
     merge.part[q] = a.part[q], merge.out[q] = dweights[q];
   }
   a.part[kGradGate] = dgate ? reinterpret_cast<float*>(ws + plan.sums_bytes + plan.weight_bytes) : nullptr;
@@ -280,7 +280,7 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
                          dim3(256), 0, st, a);
     hipLaunchKernelGGL((rn_bwd_long_apply<T>), dim3(capped(ceil_div(a.n, 2048) * a.width)), dim3(256), 0, st, a);
   }
-  if (weight_grads || dgate)
+  if ((weight_grads || dgate) && plan.ranges > 1)  // one range has written the gradients themselves
     hipLaunchKernelGGL(rn_merge, merge_grid, dim3(kMergeLanes * kMergeGroups), 0, st, merge);
   return launch_status();
 }

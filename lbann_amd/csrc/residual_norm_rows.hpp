@@ -366,6 +366,8 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
 }
 
 // ------------------------------------------------------------------ backward
+constexpr int kMergeRows = 3;
+
 // A workgroup takes a contiguous range of columns; its teams (of 16 lanes or nw waves, one unit a
 // thread) walk it with the next column's loads in flight and sum the gradients of weights and
 // gate in registers.  At the end of the range, and for several gates at the end of each gate's
@@ -386,7 +388,8 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   using U = Unit<T>;
   constexpr bool SUB = TEAM == 16;
   constexpr bool kKeepWeights = TEAM <= 512;
-  extern __shared__ float merged[];  // blockDim x 8 floats if there are several teams
+  extern __shared__ float merged[];  // kMergeRows x blockDim x 8 floats if there are several teams
+  __shared__ float* merged_rows[kMergeRows];
   __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
   const int n = static_cast<int>(a.n);
@@ -419,7 +422,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
     load_gate();
   }
 
-  float dw2[8] = {}, db2[8] = {}, dw1[8] = {}, db1[8] = {}, dg[8] = {};
+  float acc[kGrads][8] = {};
   typename U::raw_t qy{}, qh{}, qs{}, qo{};
   RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
   auto issue = [&](int64_t col) {
@@ -434,25 +437,52 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       qstats = {st[0], st[1], st[2], st[3]};  // variances, for now
     }
   };
-  // The sums of all teams, written as one row.
-  auto flush = [&](float (&acc)[8], float* row) {
+  // The sums of the quantities from FIRST to LAST whose row is given, over all teams: one row each.
+  // Several teams meet in LDS, kMergeRows rows at a time and by one piece of code for all rows (a copy
+  // of it for every quantity cost 2 us each on short ranges, in barriers and instruction fetches).
+  auto flush = [&](auto first_q, auto last_q, float* const (&rows)[kGrads]) {
+    constexpr int kFirst = decltype(first_q)::value, kLast = decltype(last_q)::value;
     if (teams == 1) {
-      store_unit<EVEN>(row + entry, valid, acc);
+#pragma unroll
+      for (int q = kFirst; q <= kLast; ++q)
+        if (rows[q]) store_unit<EVEN>(rows[q] + entry, valid, acc[q]);
     }
     else {
-      const int lanes = static_cast<int>(blockDim.x) / teams;
-      __syncthreads();  // the rows before this one have been read
+      const int lanes = static_cast<int>(blockDim.x) / teams, width = 8 * lanes;
+      auto round = [&](auto from_q, auto to_q) {
+        int count = 0;
+        __syncthreads();  // what was here has been read
 #pragma unroll
-      for (int j = 0; j < 8; ++j) merged[(team.index * lanes + team.t) * 8 + j] = acc[j];
-      __syncthreads();
-      for (int k = threadIdx.x; k < 8 * lanes && k < n; k += blockDim.x) {
-        float s = 0.f;
-        for (int i = 0; i < teams; ++i) s += merged[i * 8 * lanes + k];
-        row[k] = s;
-      }
+        for (int q = decltype(from_q)::value; q <= decltype(to_q)::value; ++q) {
+          if (rows[q]) {
+            float* mine = merged + (count * teams + team.index) * width + 8 * team.t;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mine[j] = acc[q][j];
+            if (threadIdx.x == 0) merged_rows[count] = rows[q];
+            ++count;
+          }
+        }
+        __syncthreads();
+        for (int row = 0; row < count; ++row) {
+          float* out = merged_rows[row];
+          for (int k = threadIdx.x; k < width && k < n; k += static_cast<int>(blockDim.x)) {
+            float sum = 0.f;
+            for (int i = 0; i < teams; ++i) sum += merged[(row * teams + i) * width + k];
+            out[k] = sum;
+          }
+        }
+      };
+      constexpr int kMid = kFirst + kMergeRows - 1 < kLast ? kFirst + kMergeRows - 1 : kLast;
+      round(std::integral_constant<int, kFirst>{}, std::integral_constant<int, kMid>{});
+      if constexpr (kMid < kLast) round(std::integral_constant<int, kMid + 1>{}, std::integral_constant<int, kLast>{});
     }
+  };
+  auto flush_gate = [&](int64_t gate, bool whole) {
+    float* rows[kGrads] = {};
+    rows[kGradGate] = whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (blockIdx.x + gate) * a.n;
+    flush(std::integral_constant<int, kGradGate>{}, std::integral_constant<int, kGradGate>{}, rows);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
   };
 
   bool in_flight = false;
@@ -490,8 +520,8 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             x[j] = (x[j] - s.mean2) * s.rstd2;
-            dw2[j] = __builtin_fmaf(f[j], x[j], dw2[j]);
-            if (BIAS) db2[j] += f[j];
+            acc[kGradOutputScale][j] = __builtin_fmaf(f[j], x[j], acc[kGradOutputScale][j]);
+            if (BIAS) acc[kGradOutputBias][j] += f[j];
             f[j] *= w2[j];
             sp += f[j];
             spx = __builtin_fmaf(f[j], x[j], spx);
@@ -534,7 +564,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
         if (GATE) {
           if (active && read_branch) {
             const float u = BRANCH_NORM ? (BIAS ? __builtin_fmaf(o[j], w1[j], b1[j]) : o[j] * w1[j]) : o[j];
-            dg[j] += keep[j] != 0.f ? e[j] * u : 0.f;
+            acc[kGradGate][j] += keep[j] != 0.f ? e[j] * u : 0.f;
           }
           e[j] *= gt[j];
           if (dropping) e[j] = keep[j] != 0.f ? e[j] : 0.f;
@@ -545,8 +575,8 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
         if (active) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            dw1[j] = __builtin_fmaf(e[j], o[j], dw1[j]);
-            if (BIAS) db1[j] += e[j];
+            acc[kGradBranchScale][j] = __builtin_fmaf(e[j], o[j], acc[kGradBranchScale][j]);
+            if (BIAS) acc[kGradBranchBias][j] += e[j];
             e[j] *= w1[j];
             sp += e[j];
             spu = __builtin_fmaf(e[j], o[j], spu);
@@ -562,16 +592,19 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       }
       if (active) store_unit<EVEN>(a.dbranch + col * a.ld_dbranch + entry, valid, e);
     }
-    if (GATE && a.part[kGradGate] && (several_gates || end == last)) {
-      const bool whole = begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate;
-      flush(dg, whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (blockIdx.x + gate) * a.n);
-    }
+    if (GATE && a.part[kGradGate] && several_gates)
+      flush_gate(gate, begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate);
     begin = end;
   }
-  if (a.part[kGradOutputScale]) flush(dw2, a.part[kGradOutputScale] + blockIdx.x * a.n);
-  if (BIAS && a.part[kGradOutputBias]) flush(db2, a.part[kGradOutputBias] + blockIdx.x * a.n);
-  if (BRANCH_NORM && a.part[kGradBranchScale]) flush(dw1, a.part[kGradBranchScale] + blockIdx.x * a.n);
-  if (BRANCH_NORM && BIAS && a.part[kGradBranchBias]) flush(db1, a.part[kGradBranchBias] + blockIdx.x * a.n);
+  float* rows[kGrads];
+#pragma unroll
+  for (int q = 0; q < kGrads; ++q) {
+    const bool here = q == kGradOutputScale || (q == kGradOutputBias && BIAS) || (q == kGradBranchScale && BRANCH_NORM) ||
+                      (q == kGradBranchBias && BRANCH_NORM && BIAS) || (q == kGradGate && GATE && !several_gates);
+    rows[q] = here && a.part[q] ? a.part[q] + blockIdx.x * a.n : nullptr;
+  }
+  if (GATE && !several_gates && a.part[kGradGate] && gridDim.x == 1) rows[kGradGate] = a.dgate;  // the only range
+  flush(std::integral_constant<int, 0>{}, std::integral_constant<int, kGradGate>{}, rows);
 }
 
 }  // namespace lbn
