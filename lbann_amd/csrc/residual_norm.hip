@@ -23,6 +23,8 @@
 #include "host_utils.hpp"
 #include "residual_norm_rows.hpp"
 
+#include <initializer_list>
+
 namespace lbn {
 
 // Sums the partial rows of ranges of columns: weight gradients over all ranges, a gate column
@@ -30,7 +32,9 @@ namespace lbn {
 struct RnMergeArgs {
   const float* part[kGrads];
   float* out[kGrads];
-  int64_t n, ranges, ld_dgate, num_gates, cols_per_gate, cols_per_range;
+  int64_t ld_dgate, num_gates, cols_per_gate, cols_per_range;
+  int64_t n;
+  unsigned ranges;
 };
 
 // A workgroup sums 64 neighbouring features: kMergeGroups groups of kMergeLanes lanes (four features each)
@@ -96,9 +100,22 @@ static bool rn_norm_ok(int kind) { return kind >= kNormNone && kind <= kNormLaye
 struct RnShape {
   int v, nw;
   bool sub;
-  int threads() const { return sub || nw == 1 ? 256 : kWave * nw; }
+  int threads() const { return sub || nw == 1 ? 256 : kWave * nw; }  // of a forward workgroup
   int teams() const { return sub ? 16 : (nw == 1 ? 4 : 1); }
+  RowTeams row_teams(int teams) const { return {nw, teams, static_cast<unsigned>((65536 + nw - 1) / nw)}; }
 };
+
+static unsigned ld32(int64_t ld) { return static_cast<unsigned>(ld); }
+
+// Leading dimensions (0 for a matrix that is not there) and widths that the row kernels' 32-bit indices hold.
+// A leading dimension that no second column uses is not looked at.
+static bool rn_fits32(int64_t width, std::initializer_list<int64_t> lds)
+{
+  if (width >= (int64_t(1) << 30)) return false;
+  for (int64_t ld : lds)
+    if (width > 1 && (ld < 0 || ld >= (int64_t(1) << 31))) return false;
+  return true;
+}
 
 static RnShape rn_shape(int64_t n, int max_v)
 {
@@ -139,25 +156,38 @@ static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t
   if (p.cols_per_range < p.teams) p.cols_per_range = p.teams;
   p.ranges = ceil_div(width, p.cols_per_range);
   auto round16 = [](int64_t b) { return static_cast<size_t>(ceil_div(b, 16) * 16); };
-  p.sums_bytes = p.shape.v ? 0 : round16(width * 16);
+  p.sums_bytes = round16(width * 16);  // of the long kernels, which leading dimensions may call for
   if (weight_grads) p.weight_bytes = round16(kGradGate * p.ranges * n * 4);
   if (gate_grads) p.gate_bytes = round16((p.ranges + gate_grads) * n * 4);
   return p;
 }
 
 template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN>
-static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan& plan)
+static void rn_launch_bwd(hipStream_t st, const RnBwdRows<T>& a, const RnBwdPlan& plan)
 {
   const int threads = (TEAM == 16 ? 16 : kWave * plan.shape.nw) * plan.teams;
   const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(kMergeRows * threads * 8 * sizeof(float)) : 0;
   hipLaunchKernelGGL((rn_bwd_rows<T, TEAM, BRANCH_NORM, GATE, BIAS, EVEN>), dim3(static_cast<unsigned>(plan.ranges)), dim3(threads),
-                     lds, st, a, plan.shape.nw);
+                     lds, st, a);
 }
 
 // Lengths that are no multiple of eight take the kernel that accumulates everything.
 template <typename T, int TEAM>
-static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan& plan, bool bias)
+static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& g, const RnBwdPlan& plan, bool bias)
 {
+  RnBwdRows<T> a{};
+  a.n = static_cast<int>(g.n), a.width = static_cast<int>(g.width);
+  a.branch_norm = g.branch_norm, a.output_norm = g.output_norm, a.epsilon = g.epsilon;
+  a.residual_mult = g.residual_mult, a.branch_mult = g.branch_mult;
+  a.branch = g.branch, a.h = g.h, a.dy = g.dy, a.dh = g.dh, a.gate = g.gate, a.stats = g.stats;
+  a.branch_scale = g.branch_scale, a.branch_bias = g.branch_bias, a.output_scale = g.output_scale;
+  a.dbranch = g.dbranch, a.dresidual = g.dresidual, a.dgate = g.dgate;
+  a.ld_branch = ld32(g.ld_branch), a.ld_h = ld32(g.ld_h), a.ld_dy = ld32(g.ld_dy), a.ld_dh = ld32(g.ld_dh);
+  a.ld_gate = ld32(g.ld_gate), a.ld_stats = ld32(g.ld_stats), a.ld_dgate = ld32(g.ld_dgate);
+  a.ld_dbranch = ld32(g.ld_dbranch), a.ld_dresidual = ld32(g.ld_dresidual);
+  a.cols_per_gate = static_cast<unsigned>(g.cols_per_gate), a.cols_per_range = static_cast<unsigned>(g.cols_per_range);
+  a.drop = g.drop, a.teams = plan.shape.row_teams(plan.teams);
+  for (int q = 0; q < kGrads; ++q) a.part[q] = g.part[q];
   const bool norm = a.branch_norm != kNormNone, gate = a.gate != nullptr;
   auto launch = [&](auto branch_norm) {
     constexpr bool N = decltype(branch_norm)::value;
@@ -169,12 +199,22 @@ static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& a, const RnBwdPlan
 }
 
 template <typename T, int V, bool SUB, bool EVEN>
-static void rn_launch_fwd(hipStream_t st, const RnFwdArgs<T>& a, const RnShape& shape)
+static void rn_launch_fwd(hipStream_t st, const RnFwdArgs<T>& g, const RnShape& shape)
 {
-  const int64_t blocks = ceil_div(a.width, shape.teams());
+  RnFwdRows<T> a{};
+  a.n = static_cast<int>(g.n), a.width = static_cast<int>(g.width);
+  a.branch_norm = g.branch_norm, a.output_norm = g.output_norm, a.epsilon = g.epsilon;
+  a.residual_mult = g.residual_mult, a.branch_mult = g.branch_mult;
+  a.branch = g.branch, a.residual = g.residual, a.gate = g.gate, a.h = g.h, a.y = g.y, a.stats = g.stats;
+  a.branch_scale = g.branch_scale, a.branch_bias = g.branch_bias;
+  a.output_scale = g.output_scale, a.output_bias = g.output_bias;
+  a.ld_branch = ld32(g.ld_branch), a.ld_residual = ld32(g.ld_residual), a.ld_gate = ld32(g.ld_gate);
+  a.ld_h = ld32(g.ld_h), a.ld_y = ld32(g.ld_y), a.ld_stats = ld32(g.ld_stats);
+  a.cols_per_gate = static_cast<unsigned>(g.cols_per_gate), a.drop = g.drop, a.teams = shape.row_teams(shape.teams());
+  const int64_t blocks = ceil_div(g.width, shape.teams());
   const int64_t resident = resident_blocks(rn_fwd_rows<T, V, SUB, EVEN>, shape.threads());
-  const int64_t grid = resident > 0 && blocks > resident ? resident : (blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30));
-  hipLaunchKernelGGL((rn_fwd_rows<T, V, SUB, EVEN>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads()), 0, st, a, shape.nw);
+  const int64_t grid = resident > 0 && blocks > resident ? resident : blocks;
+  hipLaunchKernelGGL((rn_fwd_rows<T, V, SUB, EVEN>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads()), 0, st, a);
 }
 
 template <typename T, bool EVEN>
@@ -206,7 +246,8 @@ static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double
   a.drop = drop_args(keep_prob, seed, offset, step, column_offset);
   hipStream_t st = as_stream(stream);
   const RnShape shape = rn_shape(a.n, 2);
-  if (shape.v) {
+  if (shape.v && rn_fits32(a.width, {a.ld_branch, a.residual ? a.ld_residual : 0, a.gate ? a.ld_gate : 0, a.h ? a.ld_h : 0,
+                                   a.y ? a.ld_y : 0, a.stats ? a.ld_stats : 0})) {
     a.n % 8 == 0 ? rn_launch_fwd<T, true>(st, a, shape) : rn_launch_fwd<T, false>(st, a, shape);
   }
   else {
@@ -246,7 +287,11 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   a.drop = drop_args(keep_prob, seed, offset, step, column_offset);
   bool weight_grads = false;
   for (float* d : dweights) weight_grads = weight_grads || d;
-  const RnBwdPlan plan = rn_bwd_plan(a.n, a.width, weight_grads, dgate ? num_gates : 0);
+  RnBwdPlan plan = rn_bwd_plan(a.n, a.width, weight_grads, dgate ? num_gates : 0);
+  if (!rn_fits32(a.width, {a.branch ? a.ld_branch : 0, a.h ? a.ld_h : 0, a.gate ? a.ld_gate : 0, a.stats ? a.ld_stats : 0,
+                           a.dy ? a.ld_dy : 0, a.dh ? a.ld_dh : 0, a.ld_dbranch, a.dresidual ? a.ld_dresidual : 0,
+                           dgate ? ld_dgate : 0}))
+    plan.shape.v = 0;
   if (plan.total() && (!workspace || workspace_bytes < plan.total() || !aligned16(workspace))) return LBN_ERR_WORKSPACE;
   char* ws = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<float*>(ws);

@@ -194,17 +194,23 @@ __device__ __forceinline__ void row_moments(const float (&x)[V][8], const RowSha
   var = q * inv_n;
 }
 
+// How a workgroup is cut into teams; `of_wave`: 65536 / nw rounded up, so that wave * of_wave >> 16 is
+// the wave's team (exact for up to 16 waves).
+struct RowTeams {
+  int nw, teams;
+  unsigned of_wave;
+};
+
 // What a team needs to know about itself; block-wide set-up of the merge buffers included.
 template <int V, bool SUB>
 struct Team {
-  int index, per_block, t;
+  int index, t;
   float inv_n, inv_mine;  // 1 / entries of the column, of this wave
-  __device__ __forceinline__ Team(int nw, int n, float2 (*slots)[kMergeSlots], TeamMerge& merge)
+  __device__ __forceinline__ Team(const RowTeams& shape, int n, float2 (*slots)[kMergeSlots], TeamMerge& merge)
   {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, nw = shape.nw;
     const int lanes = SUB ? 16 : kWave * nw;
-    per_block = static_cast<int>(blockDim.x) / lanes;
-    index = SUB ? tid / 16 : wave_index() / nw;
+    index = SUB ? tid / 16 : static_cast<int>(wave_index() * shape.of_wave >> 16);
     t = tid - index * lanes;
     merge.slots = slots;
     merge.nw = nw;
@@ -223,22 +229,59 @@ struct Team {
     inv_n = 1.f / static_cast<float>(n);
     inv_mine = inv_n;
     merge.count = 0.f;
-    if (!SUB) {
+    if (!SUB && nw > 1) {
       const int mine = entries_of(merge.wave);
       inv_mine = mine > 0 ? 1.f / static_cast<float>(mine) : 0.f;
       merge.count = (merge.lane & 15) < nw ? static_cast<float>(entries_of(merge.lane & 15)) : 0.f;
-      if (nw > 1) {
-        for (int i = tid; i < 2 * kMergeSlots; i += static_cast<int>(blockDim.x))
-          slots[i / kMergeSlots][i % kMergeSlots] = make_float2(0.f, 0.f);
-        __syncthreads();
-      }
+      for (int i = tid; i < 2 * kMergeSlots; i += static_cast<int>(blockDim.x))
+        slots[i / kMergeSlots][i % kMergeSlots] = make_float2(0.f, 0.f);
+      __syncthreads();
     }
   }
 };
 
+// The arguments of the row kernels: columns and leading dimensions in 32 bits (the host sends larger
+// ones to the long kernels).  64-bit products and divisions on the scalar unit were a third of the
+// instructions, and a kernel that walks two or three columns is bound by fetching its code: 77 ns per 64
+// bytes, 20 us for a 16 KB kernel over 777 columns of 1024.
+template <typename T>
+struct RnFwdRows {
+  int n, width;
+  int branch_norm, output_norm;
+  float epsilon, residual_mult, branch_mult;
+  const T *branch, *residual;
+  const float *gate, *branch_scale, *branch_bias, *output_scale, *output_bias;
+  T *h, *y;
+  float* stats;
+  unsigned ld_branch, ld_residual, ld_gate, ld_h, ld_y, ld_stats, cols_per_gate;
+  DropArgs drop;
+  RowTeams teams;
+};
+
+template <typename T>
+struct RnBwdRows {
+  int n, width;
+  int branch_norm, output_norm;
+  float epsilon, residual_mult, branch_mult;
+  const T *branch, *h, *dy, *dh;
+  const float *gate, *branch_scale, *branch_bias, *output_scale, *stats;
+  T *dbranch, *dresidual;
+  unsigned ld_branch, ld_h, ld_dy, ld_dh, ld_gate, ld_stats, ld_dbranch, ld_dresidual, ld_dgate, cols_per_gate, cols_per_range;
+  DropArgs drop;
+  float* part[kGrads];
+  float* dgate;
+  RowTeams teams;
+};
+
+template <typename T>
+__device__ __forceinline__ T* column(T* p, unsigned col, unsigned ld)
+{
+  return p + static_cast<uint64_t>(col) * ld;
+}
+
 template <typename T, int V, bool SUB, bool EVEN>
 __global__ void __launch_bounds__(SUB ? 256 : 1024)
-rn_fwd_rows(RnFwdArgs<T> a, int nw)
+rn_fwd_rows(RnFwdRows<T> a)
 {
   using U = Unit<T>;
   constexpr bool kKeepWeights = V == 1 || SUB;  // of a thread's units, in registers from column to column
@@ -246,14 +289,15 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   constexpr int WV = kKeepWeights ? V : 1;
   __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
-  const int n = static_cast<int>(a.n);
-  const Team<V, SUB> team(nw, n, slots, merge);
-  const RowShare<V, EVEN> share(team.t, SUB ? 16 : kWave * nw, n);
+  const int n = a.n, lanes = SUB ? 16 : kWave * a.teams.nw;
+  const Team<V, SUB> team(a.teams, n, slots, merge);
+  const RowShare<V, EVEN> share(team.t, lanes, n);
   const DropStream stream = drop_stream(a.drop);
   const bool dropping = a.drop.threshold < 65536u;
-  const bool one_gate = a.gate && a.cols_per_gate == a.width;
+  const unsigned width = a.width;
+  const bool one_gate = a.gate && a.cols_per_gate == width;
 
-  auto gate_of = [&](int64_t col) { return a.gate ? a.gate + col / a.cols_per_gate * a.ld_gate : nullptr; };
+  auto gate_of = [&](unsigned col) { return a.gate ? column(a.gate, col / a.cols_per_gate, a.ld_gate) : nullptr; };
   auto weights = [&](const float* w, int i, float fill, float (&out)[8]) { share.weights(w, i, fill, out); };
   float w1[WV][8], b1[WV][8], w2[WV][8], b2[WV][8], gt[WV][8];
   if constexpr (kKeepWeights) {
@@ -268,24 +312,24 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
   }
 
   typename U::raw_t qo[V], qr[V];
-  auto issue = [&](int64_t col) {
-    const T* o = a.branch + col * a.ld_branch;
+  auto issue = [&](unsigned col) {
+    const T* o = column(a.branch, col, a.ld_branch);
 #pragma unroll
     for (int i = 0; i < V; ++i) qo[i] = U::load(o + share.at[i]);
     if (a.residual) {
-      const T* r = a.residual + col * a.ld_residual;
+      const T* r = column(a.residual, col, a.ld_residual);
 #pragma unroll
       for (int i = 0; i < V; ++i) qr[i] = U::load(r + share.at[i]);
     }
   };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * team.per_block;
+  const unsigned step = gridDim.x * a.teams.teams;
 
   // full: every unit of every thread exists, nothing is masked
   auto walk = [&](auto full) {
     constexpr bool kFull = decltype(full)::value;
-    int64_t col = static_cast<int64_t>(blockIdx.x) * team.per_block + team.index;
-    if (kPrefetch && col < a.width) issue(col);
-    for (; col < a.width; col += step) {
+    unsigned col = blockIdx.x * a.teams.teams + team.index;
+    if (kPrefetch && col < width) issue(col);
+    for (; col < width; col += step) {
       if (!kPrefetch) issue(col);
       float x[V][8], r[V][8];
 #pragma unroll
@@ -296,11 +340,11 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
       if (a.residual) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-        if constexpr (kFull) U::widen(qr[i], r[i]);
-        else U::template widen<EVEN>(qr[i], share.shift[i], r[i]);
+          if constexpr (kFull) U::widen(qr[i], r[i]);
+          else U::template widen<EVEN>(qr[i], share.shift[i], r[i]);
+        }
       }
-      }
-      if (kPrefetch && col + step < a.width) issue(col + step);
+      if (kPrefetch && col + step < width) issue(col + step);
       if (a.gate && !one_gate && kKeepWeights) {
 #pragma unroll
         for (int i = 0; i < V; ++i) weights(gate_of(col), i, 1.f, gt[i]);
@@ -325,7 +369,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
       for (int i = 0; i < V; ++i) {
         if (dropping) {
           uint32_t w[4];
-          drop_words(a.drop, stream, share.unit[i], static_cast<uint32_t>(col), w);
+          drop_words(a.drop, stream, share.unit[i], col, w);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             x[i][j] = drop_kept(w, j, a.drop.threshold) ? x[i][j] * a.drop.inverse_keep : 0.f;
@@ -337,7 +381,7 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
           x[i][j] *= a.branch_mult * gt[kw ? i : 0][j];
           if (a.residual) x[i][j] = __builtin_fmaf(a.residual_mult, r[i][j], x[i][j]);
         }
-        if (a.h) store_unit<EVEN>(a.h + col * a.ld_h + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
+        if (a.h) store_unit<EVEN>(column(a.h, col, a.ld_h) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
       }
       if (a.output_norm != kNormNone) {
         row_moments<V, SUB, kFull, EVEN>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
@@ -352,16 +396,16 @@ rn_fwd_rows(RnFwdArgs<T> a, int nw)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             x[i][j] = __builtin_fmaf((x[i][j] - mean2) * rstd, w2[kw ? i : 0][j], b2[kw ? i : 0][j]);
-          store_unit<EVEN>(a.y + col * a.ld_y + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
+          store_unit<EVEN>(column(a.y, col, a.ld_y) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
         }
       }
       if (a.stats && team.t == 0) {
-        float* st = a.stats + col * a.ld_stats;
+        float* st = column(a.stats, col, a.ld_stats);
         st[0] = mean1, st[1] = var1, st[2] = mean2, st[3] = var2;
       }
     }
   };
-  if (EVEN && n == 8 * V * (SUB ? 16 : kWave * nw)) walk(std::integral_constant<bool, EVEN>{});
+  if (EVEN && n == 8 * V * lanes) walk(std::integral_constant<bool, EVEN>{});
   else walk(std::false_type{});
 }
 
@@ -383,7 +427,7 @@ constexpr int kMergeRows = 3;
 // every column, from L2.
 template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN>
 __global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
-rn_bwd_rows(RnBwdArgs<T> a, int nw)
+rn_bwd_rows(RnBwdRows<T> a)
 {
   using U = Unit<T>;
   constexpr bool SUB = TEAM == 16;
@@ -392,18 +436,19 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   __shared__ float* merged_rows[kMergeRows];
   __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
-  const int n = static_cast<int>(a.n);
-  const Team<1, SUB> team(nw, n, slots, merge);
-  const RowShare<1, EVEN> share(team.t, SUB ? 16 : kWave * nw, n);
+  const int n = a.n, nw = a.teams.nw, lanes = SUB ? 16 : kWave * nw;
+  const Team<1, SUB> team(a.teams, n, slots, merge);
+  const RowShare<1, EVEN> share(team.t, lanes, n);
   const int unit = share.unit[0], valid = share.valid[0], entry = 8 * unit, at = share.at[0], shift = share.shift[0];
-  const int teams = team.per_block;
+  const int teams = a.teams.teams;
   const DropStream stream = drop_stream(a.drop);
   const bool dropping = a.drop.threshold < 65536u;
-  const bool several_gates = GATE && a.cols_per_gate < a.width;
+  const unsigned width = a.width;
+  const bool several_gates = GATE && a.cols_per_gate < width;
   const bool output_norm = a.output_norm != kNormNone;
   const bool read_branch = BRANCH_NORM || (GATE && a.branch);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * a.cols_per_range;
-  const int64_t last = imin64(first + a.cols_per_range, a.width);
+  const unsigned first = blockIdx.x * a.cols_per_range;
+  const unsigned last = min(first + a.cols_per_range, width);
 
   auto weights = [&](const float* w, float fill, float (&out)[8]) { share.weights(w, 0, fill, out); };
   float w2[8], w1[8], b1[8], gt[8];
@@ -425,15 +470,15 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   float acc[kGrads][8] = {};
   typename U::raw_t qy{}, qh{}, qs{}, qo{};
   RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
-  auto issue = [&](int64_t col) {
+  auto issue = [&](unsigned col) {
     if (output_norm) {
-      qy = U::load(a.dy + col * a.ld_dy + at);
-      qs = U::load(a.h + col * a.ld_h + at);
+      qy = U::load(column(a.dy, col, a.ld_dy) + at);
+      qs = U::load(column(a.h, col, a.ld_h) + at);
     }
-    if (a.dh) qh = U::load(a.dh + col * a.ld_dh + at);
-    if (read_branch) qo = U::load(a.branch + col * a.ld_branch + at);
+    if (a.dh) qh = U::load(column(a.dh, col, a.ld_dh) + at);
+    if (read_branch) qo = U::load(column(a.branch, col, a.ld_branch) + at);
     if (BRANCH_NORM || output_norm) {
-      const float* st = a.stats + col * a.ld_stats;
+      const float* st = column(a.stats, col, a.ld_stats);
       qstats = {st[0], st[1], st[2], st[3]};  // variances, for now
     }
   };
@@ -448,14 +493,14 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
         if (rows[q]) store_unit<EVEN>(rows[q] + entry, valid, acc[q]);
     }
     else {
-      const int lanes = static_cast<int>(blockDim.x) / teams, width = 8 * lanes;
+      const int stride = 8 * lanes;
       auto round = [&](auto from_q, auto to_q) {
         int count = 0;
         __syncthreads();  // what was here has been read
 #pragma unroll
         for (int q = decltype(from_q)::value; q <= decltype(to_q)::value; ++q) {
           if (rows[q]) {
-            float* mine = merged + (count * teams + team.index) * width + 8 * team.t;
+            float* mine = merged + (count * teams + team.index) * stride + 8 * team.t;
 #pragma unroll
             for (int j = 0; j < 8; ++j) mine[j] = acc[q][j];
             if (threadIdx.x == 0) merged_rows[count] = rows[q];
@@ -465,9 +510,10 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
         __syncthreads();
         for (int row = 0; row < count; ++row) {
           float* out = merged_rows[row];
-          for (int k = threadIdx.x; k < width && k < n; k += static_cast<int>(blockDim.x)) {
+          for (int k = threadIdx.x; k < n; k += static_cast<int>(blockDim.x)) {
             float sum = 0.f;
-            for (int i = 0; i < teams; ++i) sum += merged[(row * teams + i) * width + k];
+#pragma unroll 1
+            for (int i = 0; i < teams; ++i) sum += merged[(row * teams + i) * stride + k];
             out[k] = sum;
           }
         }
@@ -477,27 +523,26 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       if constexpr (kMid < kLast) round(std::integral_constant<int, kMid + 1>{}, std::integral_constant<int, kLast>{});
     }
   };
-  auto flush_gate = [&](int64_t gate, bool whole) {
+  auto flush_gate = [&](unsigned gate, bool whole) {
     float* rows[kGrads] = {};
-    rows[kGradGate] = whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (blockIdx.x + gate) * a.n;
+    rows[kGradGate] = whole ? column(a.dgate, gate, a.ld_dgate) : column(a.part[kGradGate], blockIdx.x + gate, n);
     flush(std::integral_constant<int, kGradGate>{}, std::integral_constant<int, kGradGate>{}, rows);
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
   };
 
   bool in_flight = false;
-  for (int64_t begin = first; begin < last;) {
-    int64_t end = last, gate = 0;
+  for (unsigned begin = first; begin < last;) {
+    unsigned end = last, gate = 0;
     if (several_gates) {
       gate = begin / a.cols_per_gate;
-      end = imin64(last, (gate + 1) * a.cols_per_gate);
-      gate_row = a.gate + gate * a.ld_gate;
+      end = min(last, (gate + 1) * a.cols_per_gate);
+      gate_row = column(a.gate, gate, a.ld_gate);
       if (kKeepWeights) load_gate();
     }
-    const int64_t turns = (end - begin + teams - 1) / teams;
-    int64_t col = begin + team.index;
+    unsigned col = begin + team.index;
     if (!in_flight && col < end) issue(col);
-    for (int64_t turn = 0; turn < turns; ++turn, col += teams) {
+    for (unsigned turn = begin; turn < end; turn += teams, col += teams) {
       const bool active = col < end;
       float e[8], f[8], x[8];
       RnColumnStats s = qstats;
@@ -509,7 +554,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       U::template widen<EVEN>(qh, shift, e);
       U::template widen<EVEN>(qo, shift, o);
       // a single team carries the next column over the end of a gate's columns
-      const int64_t next = col + teams;
+      const unsigned next = col + teams;
       in_flight = teams == 1 && next < last;
       if (in_flight || next < end) issue(next);
 
@@ -538,37 +583,38 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
       if (active && a.dresidual) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = a.residual_mult * e[j];
-        store_unit<EVEN>(a.dresidual + col * a.ld_dresidual + entry, valid, f);
+        store_unit<EVEN>(column(a.dresidual, col, a.ld_dresidual) + entry, valid, f);
       }
       // e becomes du; o the normalised branch
       if constexpr (!kKeepWeights) {
         load_branch_weights();
         load_gate();
       }
-      float keep[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) keep[j] = 1.f;
-      if (dropping) {
-        uint32_t w[4];
-        drop_words(a.drop, stream, unit, static_cast<uint32_t>(col), w);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) keep[j] = drop_kept(w, j, a.drop.threshold) ? a.drop.inverse_keep : 0.f;
-      }
-      if (BRANCH_NORM) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = (o[j] - s.mean1) * s.rstd1;
-      }
+      const float scale = dropping ? a.branch_mult * a.drop.inverse_keep : a.branch_mult;
+      float ev[8];  // the gate's gradient
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        e[j] = keep[j] != 0.f ? a.branch_mult * e[j] * keep[j] : 0.f;
+        if (BRANCH_NORM) o[j] = (o[j] - s.mean1) * s.rstd1;
+        e[j] *= scale;
         if (GATE) {
-          if (active && read_branch) {
-            const float u = BRANCH_NORM ? (BIAS ? __builtin_fmaf(o[j], w1[j], b1[j]) : o[j] * w1[j]) : o[j];
-            acc[kGradGate][j] += keep[j] != 0.f ? e[j] * u : 0.f;
-          }
+          const float u = BRANCH_NORM ? (BIAS ? __builtin_fmaf(o[j], w1[j], b1[j]) : o[j] * w1[j]) : o[j];
+          ev[j] = e[j] * u;
           e[j] *= gt[j];
-          if (dropping) e[j] = keep[j] != 0.f ? e[j] : 0.f;
         }
+      }
+      if (dropping) {
+        uint32_t w[4];
+        drop_words(a.drop, stream, unit, col, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool kept = drop_kept(w, j, a.drop.threshold);
+          e[j] = kept ? e[j] : 0.f;
+          if (GATE) ev[j] = kept ? ev[j] : 0.f;
+        }
+      }
+      if (GATE && active && read_branch) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[kGradGate][j] += ev[j];
       }
       if (BRANCH_NORM) {
         float sp = 0.f, spu = 0.f;
@@ -590,7 +636,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = s.rstd1 * (e[j] - sp - o[j] * spu);
       }
-      if (active) store_unit<EVEN>(a.dbranch + col * a.ld_dbranch + entry, valid, e);
+      if (active) store_unit<EVEN>(column(a.dbranch, col, a.ld_dbranch) + entry, valid, e);
     }
     if (GATE && a.part[kGradGate] && several_gates)
       flush_gate(gate, begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate);
@@ -601,7 +647,7 @@ rn_bwd_rows(RnBwdArgs<T> a, int nw)
   for (int q = 0; q < kGrads; ++q) {
     const bool here = q == kGradOutputScale || (q == kGradOutputBias && BIAS) || (q == kGradBranchScale && BRANCH_NORM) ||
                       (q == kGradBranchBias && BRANCH_NORM && BIAS) || (q == kGradGate && GATE && !several_gates);
-    rows[q] = here && a.part[q] ? a.part[q] + blockIdx.x * a.n : nullptr;
+    rows[q] = here && a.part[q] ? column(a.part[q], blockIdx.x, n) : nullptr;
   }
   if (GATE && !several_gates && a.part[kGradGate] && gridDim.x == 1) rows[kGradGate] = a.dgate;  // the only range
   flush(std::integral_constant<int, 0>{}, std::integral_constant<int, kGradGate>{}, rows);
