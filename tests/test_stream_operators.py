@@ -150,6 +150,7 @@ def test_logits_adjust_refusals(suffix):
                 dict(m=None), dict(ldm=3), dict(index=None)):
         assert call(**bad) == INVALID, bad
     assert call(v=2 ** 31, ldx=2 ** 31, ldy=2 ** 31, ldm=2 ** 26) == UNSUPPORTED
+    assert call(most=131072, ldt=131072, k=8192, ldbt=8192, ldbv=8192) == UNSUPPORTED
 
 
 def test_layer_classes_refuse():
