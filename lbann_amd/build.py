@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "liblbnorm.so")
 SOURCES = ["capi_common.hip", "softmax.hip", "layer_norm.hip", "batch_norm.hip", "entrywise_batch_norm.hip",
            "entrywise_batch_norm_split.hip", "cross_entropy.hip", "scale_bias.hip", "gradient_sink.hip", "f64_layers.hip",
-           "dropout.hip", "residual_norm.hip", "logits_adjust.hip"]
+           "dropout.hip", "residual_norm_f32.hip", "residual_norm_f16.hip", "residual_norm_bf16.hip", "logits_adjust.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -24,6 +24,21 @@ template <typename T>
 struct Unit {
   typedef T raw_t __attribute__((ext_vector_type(8), aligned(sizeof(T))));
   static __device__ __forceinline__ raw_t load(const T* p) { return *reinterpret_cast<const raw_t*>(p); }
+  // STREAM: past the caches, for calls that move more than they hold.
+  template <bool STREAM>
+  static __device__ __forceinline__ raw_t load(const T* p)
+  {
+    if constexpr (!STREAM) return load(p);
+    constexpr int N = Pack<T>::N;
+    raw_t r;
+#pragma unroll
+    for (int i = 0; i < 8; i += N) {
+      const typename Pack<T>::vec_t v = __builtin_nontemporal_load(reinterpret_cast<const typename Pack<T>::vec_t*>(p + i));
+#pragma unroll
+      for (int k = 0; k < N; ++k) r[i + k] = v[k];
+    }
+    return r;
+  }
   static __device__ __forceinline__ raw_t moved(const raw_t& r, int shift)
   {
     constexpr int W = 2 * static_cast<int>(sizeof(T));  // words of a unit
@@ -75,23 +90,25 @@ struct Unit {
 };
 
 // Eight entries in the storage type: the whole unit, or its first `valid` ones in up to three pieces.
+// Ordinary stores: what these kernels write is read next, and as long as it fits the last-level
+// cache it stays there (backward, 4096 x 8192 bf16 with streamed loads: 76.5 us against 86.0 with
+// non-temporal stores; forward 44.6 against 48.7).
 template <bool EVEN, typename T>
 __device__ __forceinline__ void store_unit(T* p, int valid, const float (&v)[8])
 {
+  T t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = static_cast<T>(v[j]);
   if (valid == 8) {
-    store8(p, 8, v);
+    __builtin_memcpy(p, t, sizeof(t));
   }
   else if constexpr (!EVEN) {
-    T t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = static_cast<T>(v[j]);
-    typedef T four_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-    typedef T two_t __attribute__((ext_vector_type(2), aligned(sizeof(T))));
     const bool four = valid & 4, two = valid & 2;
-    if (four) *reinterpret_cast<four_t*>(p) = four_t{t[0], t[1], t[2], t[3]};
-    T a = four ? t[4] : t[0], b = four ? t[5] : t[1], c = four ? t[6] : t[2];
-    if (two) *reinterpret_cast<two_t*>(p + (valid & 4)) = two_t{a, b};
-    if (valid & 1) p[valid & 6] = two ? c : a;
+    if (four) __builtin_memcpy(p, t, 4 * sizeof(T));
+    const T a[2] = {four ? t[4] : t[0], four ? t[5] : t[1]};
+    const T c = four ? t[6] : t[2];
+    if (two) __builtin_memcpy(p + (valid & 4), a, 2 * sizeof(T));
+    if (valid & 1) p[valid & 6] = two ? c : a[0];
   }
 }
 
@@ -279,7 +296,7 @@ __device__ __forceinline__ T* column(T* p, unsigned col, unsigned ld)
   return p + static_cast<uint64_t>(col) * ld;
 }
 
-template <typename T, int V, bool SUB, bool EVEN>
+template <typename T, int V, bool SUB, bool EVEN, bool STREAM>
 __global__ void __launch_bounds__(SUB ? 256 : 1024)
 rn_fwd_rows(RnFwdRows<T> a)
 {
@@ -315,11 +332,11 @@ rn_fwd_rows(RnFwdRows<T> a)
   auto issue = [&](unsigned col) {
     const T* o = column(a.branch, col, a.ld_branch);
 #pragma unroll
-    for (int i = 0; i < V; ++i) qo[i] = U::load(o + share.at[i]);
+    for (int i = 0; i < V; ++i) qo[i] = U::template load<STREAM>(o + share.at[i]);
     if (a.residual) {
       const T* r = column(a.residual, col, a.ld_residual);
 #pragma unroll
-      for (int i = 0; i < V; ++i) qr[i] = U::load(r + share.at[i]);
+      for (int i = 0; i < V; ++i) qr[i] = U::template load<STREAM>(r + share.at[i]);
     }
   };
   const unsigned step = gridDim.x * a.teams.teams;
@@ -400,8 +417,8 @@ rn_fwd_rows(RnFwdRows<T> a)
         }
       }
       if (a.stats && team.t == 0) {
-        float* st = column(a.stats, col, a.ld_stats);
-        st[0] = mean1, st[1] = var1, st[2] = mean2, st[3] = var2;
+        const float st[4] = {mean1, var1, mean2, var2};
+        __builtin_memcpy(column(a.stats, col, a.ld_stats), st, sizeof(st));
       }
     }
   };
@@ -417,7 +434,7 @@ constexpr int kMergeRows = 3;
 // gate in registers.  At the end of the range, and for several gates at the end of each gate's
 // columns, the teams' sums are merged through LDS and leave one partial row.
 // BRANCH_NORM, GATE, BIAS: what there is to accumulate (BIAS: of any norm); GATE and BIAS may be
-// set where there is none.  EVEN: the length is a multiple of eight.
+// set where there is none.  EVEN: the length is a multiple of eight.  STREAM: inputs past the caches.
 //
 // Entries that do not exist are loaded as zeros and have zero weights, so that they add nothing
 // to any sum and need no masks.
@@ -425,7 +442,7 @@ constexpr int kMergeRows = 3;
 // TEAM: lanes of the largest team.  Up to 512 (256 registers a thread) the weights of a thread's unit stay in
 // registers beside its up to five sums; teams of up to 1024 (128 registers) read them again for
 // every column, from L2.
-template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN>
+template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN, bool STREAM>
 __global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
 rn_bwd_rows(RnBwdRows<T> a)
 {
@@ -472,11 +489,11 @@ rn_bwd_rows(RnBwdRows<T> a)
   RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
   auto issue = [&](unsigned col) {
     if (output_norm) {
-      qy = U::load(column(a.dy, col, a.ld_dy) + at);
-      qs = U::load(column(a.h, col, a.ld_h) + at);
+      qy = U::template load<STREAM>(column(a.dy, col, a.ld_dy) + at);
+      qs = U::template load<STREAM>(column(a.h, col, a.ld_h) + at);
     }
-    if (a.dh) qh = U::load(column(a.dh, col, a.ld_dh) + at);
-    if (read_branch) qo = U::load(column(a.branch, col, a.ld_branch) + at);
+    if (a.dh) qh = U::template load<STREAM>(column(a.dh, col, a.ld_dh) + at);
+    if (read_branch) qo = U::template load<STREAM>(column(a.branch, col, a.ld_branch) + at);
     if (BRANCH_NORM || output_norm) {
       const float* st = column(a.stats, col, a.ld_stats);
       qstats = {st[0], st[1], st[2], st[3]};  // variances, for now
