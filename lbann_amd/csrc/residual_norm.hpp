@@ -139,27 +139,35 @@ struct RnBwdPlan {
   RnShape shape;  // v == 0: the long kernels
   int teams;
   int64_t ranges, cols_per_range;
+  bool twice;  // two workgroups a compute unit, where the kernel's registers allow it
   size_t sums_bytes, weight_bytes, gate_bytes;
   size_t total() const { return sums_bytes + weight_bytes + gate_bytes; }
+  int threads() const { return (shape.sub ? 16 : kWave * shape.nw) * teams; }
+  void cut(int64_t width, int64_t most)
+  {
+    cols_per_range = ceil_div(width, most);
+    if (cols_per_range < teams) cols_per_range = teams;
+    ranges = ceil_div(width, cols_per_range);
+  }
 };
+
+// One workgroup a compute unit, which keeps the partial rows few: 256 ranges of columns.  Where its
+// teams leave a quarter of its lanes or more without entries, two (33.5 M entries, bf16: 256 features 76
+// -> 65 us, 3000 features 73 -> 64, but 4096 features 59 -> 61).
+constexpr int64_t kRnRanges = 256;
 
 static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t gate_grads)
 {
   RnBwdPlan p{};
   p.shape = rn_shape(n);
-  constexpr int64_t kRanges = 256;  // one workgroup per compute unit
+  p.teams = 1;
   if (p.shape.v == 1) {
     // a workgroup of up to 8 waves (16 for the widest teams), as many teams as leave a column for every workgroup
-    const int64_t most = p.shape.sub ? 32 : (p.shape.nw <= 8 ? 8 / p.shape.nw : 1);
-    p.teams = static_cast<int>(most);
-    while (p.teams > (p.shape.sub ? 4 : 1) && width < kRanges * p.teams) p.teams = p.shape.sub ? p.teams / 2 : p.teams - 1;
+    p.teams = p.shape.sub ? 32 : (p.shape.nw <= 8 ? 8 / p.shape.nw : 1);
+    while (p.teams > (p.shape.sub ? 4 : 1) && width < kRnRanges * p.teams) p.teams = p.shape.sub ? p.teams / 2 : p.teams - 1;
+    p.twice = p.shape.nw <= 8 && ceil_div(n, 8) * p.teams <= 384;
   }
-  else {
-    p.teams = 1;
-  }
-  p.cols_per_range = ceil_div(width, kRanges);
-  if (p.cols_per_range < p.teams) p.cols_per_range = p.teams;
-  p.ranges = ceil_div(width, p.cols_per_range);
+  p.cut(width, p.twice ? 2 * kRnRanges : kRnRanges);
   auto round16 = [](int64_t b) { return static_cast<size_t>(ceil_div(b, 16) * 16); };
   p.sums_bytes = round16(width * 16);  // of the long kernels, which leading dimensions may call for
   if (weight_grads) p.weight_bytes = round16(kGradGate * p.ranges * n * 4);
@@ -167,18 +175,33 @@ static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t
   return p;
 }
 
-template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN, bool STREAM>
-static void rn_launch_bwd(hipStream_t st, const RnBwdRows<T>& a, const RnBwdPlan& plan)
+// The row kernel of a call.  Lengths that are no multiple of eight take the one that accumulates everything.
+template <typename T, int TEAM>
+static auto rn_bwd_kernel(bool norm, bool gate, bool bias, bool even, bool stream) -> void (*)(RnBwdRows<T>)
 {
-  const int threads = (TEAM == 16 ? 16 : kWave * plan.shape.nw) * plan.teams;
-  const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(kMergeRows * threads * 8 * sizeof(float)) : 0;
-  hipLaunchKernelGGL((rn_bwd_rows<T, TEAM, BRANCH_NORM, GATE, BIAS, EVEN, STREAM>), dim3(static_cast<unsigned>(plan.ranges)), dim3(threads),
-                     lds, st, a);
+  auto of = [&](auto n, auto s) -> void (*)(RnBwdRows<T>) {
+    constexpr bool N = decltype(n)::value, S = decltype(s)::value;
+    if (gate) return bias ? rn_bwd_rows<T, TEAM, N, true, true, true, S> : rn_bwd_rows<T, TEAM, N, true, false, true, S>;
+    return bias ? rn_bwd_rows<T, TEAM, N, false, true, true, S> : rn_bwd_rows<T, TEAM, N, false, false, true, S>;
+  };
+  if (!even) return norm ? rn_bwd_rows<T, TEAM, true, true, true, false, false> : rn_bwd_rows<T, TEAM, false, true, true, false, false>;
+  if (stream) return norm ? of(std::true_type{}, std::true_type{}) : of(std::false_type{}, std::true_type{});
+  return norm ? of(std::true_type{}, std::false_type{}) : of(std::false_type{}, std::false_type{});
 }
 
-// Lengths that are no multiple of eight take the kernel that accumulates everything.
-template <typename T, int TEAM>
-static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& g, const RnBwdPlan& plan, bool bias)
+template <typename T>
+static auto rn_bwd_kernel(const RnBwdArgs<T>& g, const RnShape& shape, bool bias) -> void (*)(RnBwdRows<T>)
+{
+  const bool norm = g.branch_norm != kNormNone, gate = g.gate != nullptr, even = g.n % 8 == 0;
+  const int64_t bytes = g.n * g.width * static_cast<int64_t>(sizeof(T)) * (1 + 2 * !!g.dy + !!g.dh + !!g.branch + !!g.dresidual);
+  const bool stream = stream_call_inputs(bytes, kRnStreamBytes);
+  if (shape.sub) return rn_bwd_kernel<T, 16>(norm, gate, bias, even, stream);
+  if (shape.nw <= 8) return rn_bwd_kernel<T, 512>(norm, gate, bias, even, stream);
+  return rn_bwd_kernel<T, 1024>(norm, gate, bias, even, stream);
+}
+
+template <typename T>
+static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& g, const RnBwdPlan& plan, void (*kernel)(RnBwdRows<T>))
 {
   RnBwdRows<T> a{};
   a.n = static_cast<int>(g.n), a.width = static_cast<int>(g.width);
@@ -193,19 +216,8 @@ static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& g, const RnBwdPlan
   a.cols_per_gate = static_cast<unsigned>(g.cols_per_gate), a.cols_per_range = static_cast<unsigned>(g.cols_per_range);
   a.drop = g.drop, a.teams = plan.shape.row_teams(plan.teams);
   for (int q = 0; q < kGrads; ++q) a.part[q] = g.part[q];
-  const bool norm = a.branch_norm != kNormNone, gate = a.gate != nullptr;
-  const int64_t bytes = g.n * g.width * static_cast<int64_t>(sizeof(T)) * (1 + 2 * !!g.dy + !!g.dh + !!g.branch + !!g.dresidual);
-  auto launch = [&](auto branch_norm, auto stream) {
-    constexpr bool N = decltype(branch_norm)::value, S = decltype(stream)::value;
-    if (gate) bias ? rn_launch_bwd<T, TEAM, N, true, true, true, S>(st, a, plan) : rn_launch_bwd<T, TEAM, N, true, false, true, S>(st, a, plan);
-    else bias ? rn_launch_bwd<T, TEAM, N, false, true, true, S>(st, a, plan) : rn_launch_bwd<T, TEAM, N, false, false, true, S>(st, a, plan);
-  };
-  if (a.n % 8)
-    norm ? rn_launch_bwd<T, TEAM, true, true, true, false, false>(st, a, plan) : rn_launch_bwd<T, TEAM, false, true, true, false, false>(st, a, plan);
-  else if (stream_call_inputs(bytes, kRnStreamBytes))
-    norm ? launch(std::true_type{}, std::true_type{}) : launch(std::false_type{}, std::true_type{});
-  else
-    norm ? launch(std::true_type{}, std::false_type{}) : launch(std::false_type{}, std::false_type{});
+  const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(kMergeRows * plan.threads() * 8 * sizeof(float)) : 0;
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(plan.ranges)), dim3(plan.threads()), lds, st, a);
 }
 
 template <typename T, int V, bool SUB, bool EVEN, bool STREAM>
@@ -308,6 +320,12 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
                            dgate ? ld_dgate : 0}))
     plan.shape.v = 0;
   if (plan.total() && (!workspace || workspace_bytes < plan.total() || !aligned16(workspace))) return LBN_ERR_WORKSPACE;
+  void (*kernel)(RnBwdRows<T>) = nullptr;
+  if (plan.shape.v) {
+    const bool bias = dweights[kGradOutputBias] || dweights[kGradBranchBias] || (dgate && a.branch_bias);
+    kernel = rn_bwd_kernel<T>(a, plan.shape, bias);
+    if (plan.twice && resident_blocks(kernel, plan.threads()) < 2 * kRnRanges) plan.cut(a.width, kRnRanges);
+  }
   char* ws = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<float*>(ws);
   a.cols_per_range = plan.cols_per_range;
@@ -328,10 +346,7 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
 
   hipStream_t st = as_stream(stream);
   if (plan.shape.v) {
-    const bool bias = dweights[kGradOutputBias] || dweights[kGradBranchBias] || (dgate && a.branch_bias);
-    if (plan.shape.sub) rn_launch_bwd<T, 16>(st, a, plan, bias);
-    else if (plan.shape.nw <= 8) rn_launch_bwd<T, 512>(st, a, plan, bias);
-    else rn_launch_bwd<T, 1024>(st, a, plan, bias);
+    rn_launch_bwd<T>(st, a, plan, kernel);
   }
   else {
     hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(capped(a.width)), dim3(kRnLongThreads), 0, st, a);

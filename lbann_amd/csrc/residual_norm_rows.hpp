@@ -90,17 +90,19 @@ struct Unit {
 };
 
 // Eight entries in the storage type: the whole unit, or its first `valid` ones in up to three pieces.
-// Ordinary stores: what these kernels write is read next, and as long as it fits the last-level
-// cache it stays there (backward, 4096 x 8192 bf16 with streamed loads: 76.5 us against 86.0 with
-// non-temporal stores; forward 44.6 against 48.7).
-template <bool EVEN, typename T>
+// NT: past the caches, for forward calls that are themselves too large for them: a training step writes
+// its activations to fresh memory (4096 x 8192 bf16, eight sets of outputs in turn: 47.5 us, 50.7 with
+// ordinary stores).  Gradients are read next and their memory soon used again: ordinary stores
+// keep them in the last-level cache (backward of the same shape: 76.5 us against 86.0).
+template <bool EVEN, bool NT = false, typename T>
 __device__ __forceinline__ void store_unit(T* p, int valid, const float (&v)[8])
 {
   T t[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) t[j] = static_cast<T>(v[j]);
   if (valid == 8) {
-    __builtin_memcpy(p, t, sizeof(t));
+    if constexpr (NT) store8(p, 8, v);
+    else __builtin_memcpy(p, t, sizeof(t));
   }
   else if constexpr (!EVEN) {
     const bool four = valid & 4, two = valid & 2;
@@ -398,7 +400,7 @@ rn_fwd_rows(RnFwdRows<T> a)
           x[i][j] *= a.branch_mult * gt[kw ? i : 0][j];
           if (a.residual) x[i][j] = __builtin_fmaf(a.residual_mult, r[i][j], x[i][j]);
         }
-        if (a.h) store_unit<EVEN>(column(a.h, col, a.ld_h) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
+        if (a.h) store_unit<EVEN, STREAM>(column(a.h, col, a.ld_h) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
       }
       if (a.output_norm != kNormNone) {
         row_moments<V, SUB, kFull, EVEN>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
@@ -413,7 +415,7 @@ rn_fwd_rows(RnFwdRows<T> a)
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             x[i][j] = __builtin_fmaf((x[i][j] - mean2) * rstd, w2[kw ? i : 0][j], b2[kw ? i : 0][j]);
-          store_unit<EVEN>(column(a.y, col, a.ld_y) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
+          store_unit<EVEN, STREAM>(column(a.y, col, a.ld_y) + 8 * share.unit[i], kFull ? 8 : share.valid[i], x[i]);
         }
       }
       if (a.stats && team.t == 0) {
@@ -440,15 +442,15 @@ constexpr int kMergeRows = 3;
 // to any sum and need no masks.
 //
 // TEAM: lanes of the largest team.  Up to 512 (256 registers a thread) the weights of a thread's unit stay in
-// registers beside its up to five sums; teams of up to 1024 (128 registers) read them again for
-// every column, from L2.
+// registers beside its up to five sums; teams of up to 1024 (128 registers) with many sums read them
+// again for every column, from L2.
 template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN, bool STREAM>
 __global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
 rn_bwd_rows(RnBwdRows<T> a)
 {
   using U = Unit<T>;
   constexpr bool SUB = TEAM == 16;
-  constexpr bool kKeepWeights = TEAM <= 512;
+  constexpr bool kKeepWeights = TEAM <= 512 || (!GATE && (sizeof(T) == 2 ? !(BRANCH_NORM && BIAS) : !BRANCH_NORM));
   extern __shared__ float merged[];  // kMergeRows x blockDim x 8 floats if there are several teams
   __shared__ float* merged_rows[kMergeRows];
   __shared__ float2 slots[2][kMergeSlots];
