@@ -14,11 +14,10 @@
 //   p1 = du scale1;     do = rstd1 (p1 - mean(p1) - uh mean(p1 uh))
 //   dscale2 = sum dy xh, dbias2 = sum dy, dscale1 = sum du uh, dbias1 = sum du
 //
-// (the RMS norm drops mean(p)).  Sums over columns go through partial rows in the workspace,
-// merged in a fixed order: no atomics, bitwise reproducible.  A gate column is shared by
-// width / num_gates consecutive columns; a range of columns leaves one partial row per gate it
-// meets, and range b and gate g use row b + g: ranges and gates are both contiguous, so b + g
-// grows from one pair to the next and no row is used twice.
+// (the RMS norm drops mean(p)).  Sums over columns go through partial rows in the workspace, one for
+// every range of columns, merged in a fixed order: no atomics, bitwise reproducible.  A gate column
+// is shared by width / num_gates consecutive columns; ranges either lie within one gate's columns
+// or hold all columns of the gates they meet.
 #pragma once
 
 #include "device_utils.hpp"
@@ -30,13 +29,12 @@
 namespace lbn {
 
 // Sums the partial rows of ranges of columns: weight gradients over all ranges, a gate column
-// over the ranges that meet it.
+// over its own.
 struct RnMergeArgs {
   const float* part[kGrads];
   float* out[kGrads];
-  int64_t ld_dgate, num_gates, cols_per_gate, cols_per_range;
-  int64_t n;
-  unsigned ranges;
+  int64_t n, ld_dgate;
+  unsigned ranges, num_gates, ranges_per_gate;
 };
 
 // A workgroup sums 64 neighbouring features: kMergeGroups groups of kMergeLanes lanes (four features each)
@@ -51,36 +49,39 @@ rn_merge(RnMergeArgs a)
   __shared__ float sums[kMergeGroups][4 * kMergeLanes + 4];
   const int lane = threadIdx.x % kMergeLanes, group = threadIdx.x / kMergeLanes;
   const int64_t first_k = static_cast<int64_t>(blockIdx.x) * 4 * kMergeLanes, k = first_k + 4 * lane;
-  for (int64_t item = blockIdx.y; item < kGradGate + a.num_gates; item += gridDim.y) {
+  for (uint64_t item = blockIdx.y; item < uint64_t(kGradGate) + a.num_gates; item += gridDim.y) {
     const int q = item < kGradGate ? static_cast<int>(item) : kGradGate;
     if (!a.out[q]) continue;
-    const int64_t gate = item - kGradGate;  // the partial rows from `first` to `last`
-    int64_t first = 0, last = a.ranges - 1;
+    const unsigned gate = static_cast<unsigned>(item) - kGradGate;  // the partial rows from `first` to `last`
+    uint64_t first = 0, last = a.ranges - 1;
     float* out = a.out[q];
     if (q == kGradGate) {
-      first = gate * a.cols_per_gate / a.cols_per_range;
-      last = ((gate + 1) * a.cols_per_gate - 1) / a.cols_per_range;
-      if (first == last) continue;  // written by the range that holds it
-      first += gate, last += gate;
+      first = static_cast<uint64_t>(gate) * a.ranges_per_gate;
+      last = first + a.ranges_per_gate - 1;
       out += gate * a.ld_dgate;
     }
-    float s[4] = {};
-    if (k + 4 <= a.n) {
+    // The last features are read from further back, so that every read is whole: lanes that overlap
+    // then write the same sums.
+    const int64_t from = k + 4 <= a.n ? k : a.n - 4;
+    if (k < a.n && from >= 0) {
+      float s[4] = {};
 #pragma unroll 4
-      for (int64_t b = first + group; b <= last; b += kMergeGroups) {
-        const typename Pack<float>::vec_t r = Pack<float>::load(a.part[q] + b * a.n + k);
+      for (uint64_t b = first + group; b <= last; b += kMergeGroups) {
+        const typename Pack<float>::vec_t r = Pack<float>::load(a.part[q] + b * a.n + from);
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[j] += r[j];
       }
-    }
-    else {
-      for (int64_t b = first + group; b <= last; b += kMergeGroups)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (k + j < a.n) s[j] += a.part[q][b * a.n + k + j];
+      for (int j = 0; j < 4; ++j)
+        if (from + j >= first_k) sums[group][from - first_k + j] = s[j];
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) sums[group][4 * lane + j] = s[j];
+    else if (k < a.n) {  // fewer than four features
+      for (int j = 0; j < a.n; ++j) {
+        float s = 0.f;
+        for (uint64_t b = first + group; b <= last; b += kMergeGroups) s += a.part[q][b * a.n + j];
+        sums[group][j] = s;
+      }
+    }
     __syncthreads();
     // sixteen threads a feature, four groups each, then a row of lanes
     const int feature = threadIdx.x / 16, part = threadIdx.x % 16;
@@ -138,15 +139,27 @@ static RnShape rn_shape(int64_t n, int max_v = 1)
 struct RnBwdPlan {
   RnShape shape;  // v == 0: the long kernels
   int teams;
-  int64_t ranges, cols_per_range;
+  int64_t ranges, cols_per_range, ranges_per_gate;
   bool twice;  // two workgroups a compute unit, where the kernel's registers allow it
   size_t sums_bytes, weight_bytes, gate_bytes;
   size_t total() const { return sums_bytes + weight_bytes + gate_bytes; }
   int threads() const { return (shape.sub ? 16 : kWave * shape.nw) * teams; }
-  void cut(int64_t width, int64_t most)
+  // About `most` ranges that do not cut across the end of a gate's columns.
+  void cut(int64_t width, int64_t gates, int64_t most)
   {
     cols_per_range = ceil_div(width, most);
     if (cols_per_range < teams) cols_per_range = teams;
+    ranges_per_gate = 0;
+    if (gates > 0) {
+      const int64_t per_gate = width / gates;
+      if (per_gate > cols_per_range) {
+        ranges_per_gate = ceil_div(per_gate, cols_per_range);
+        cols_per_range = ceil_div(per_gate, ranges_per_gate);
+        ranges = gates * ranges_per_gate;
+        return;
+      }
+      cols_per_range = ceil_div(cols_per_range, per_gate) * per_gate;
+    }
     ranges = ceil_div(width, cols_per_range);
   }
 };
@@ -156,22 +169,34 @@ struct RnBwdPlan {
 // -> 65 us, 3000 features 73 -> 64, but 4096 features 59 -> 61).
 constexpr int64_t kRnRanges = 256;
 
+// gate_grads: the number of gates whose gradient is wanted.
 static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t gate_grads)
 {
   RnBwdPlan p{};
   p.shape = rn_shape(n);
   p.teams = 1;
+  int64_t most_ranges = kRnRanges;
   if (p.shape.v == 1) {
-    // a workgroup of up to 8 waves (16 for the widest teams), as many teams as leave a column for every workgroup
-    p.teams = p.shape.sub ? 32 : (p.shape.nw <= 8 ? 8 / p.shape.nw : 1);
-    while (p.teams > (p.shape.sub ? 4 : 1) && width < kRnRanges * p.teams) p.teams = p.shape.sub ? p.teams / 2 : p.teams - 1;
-    p.twice = p.shape.nw <= 8 && ceil_div(n, 8) * p.teams <= 384;
+    // a workgroup of up to 8 waves (16 for the widest teams), no more teams than its range has columns
+    const int64_t columns = ceil_div(width, kRnRanges);
+    if (gate_grads > 1 && width / gate_grads < 16) {
+      // few columns a gate: teams would wait for each other at the end of each, so single ones, more of them
+      p.shape.sub = false;
+      most_ranges = kRnRanges * (p.shape.nw <= 2 ? 4 : p.shape.nw <= 4 ? 2 : 1);
+    }
+    else {
+      const int64_t most = p.shape.sub ? 32 : (p.shape.nw <= 8 ? 8 / p.shape.nw : 1);
+      p.teams = static_cast<int>(columns < most ? columns : most);
+      if (p.shape.sub) p.teams = static_cast<int>(ceil_div(p.teams, 4) * 4);  // whole waves
+      p.twice = p.shape.nw <= 8 && ceil_div(n, 8) * p.teams <= 384;
+      if (p.twice) most_ranges = 2 * kRnRanges;
+    }
   }
-  p.cut(width, p.twice ? 2 * kRnRanges : kRnRanges);
+  p.cut(width, gate_grads, most_ranges);
   auto round16 = [](int64_t b) { return static_cast<size_t>(ceil_div(b, 16) * 16); };
   p.sums_bytes = round16(width * 16);  // of the long kernels, which leading dimensions may call for
   if (weight_grads) p.weight_bytes = round16(kGradGate * p.ranges * n * 4);
-  if (gate_grads) p.gate_bytes = round16((p.ranges + gate_grads) * n * 4);
+  if (gate_grads && p.ranges_per_gate) p.gate_bytes = round16(p.ranges * n * 4);
   return p;
 }
 
@@ -214,6 +239,7 @@ static void rn_launch_bwd(hipStream_t st, const RnBwdArgs<T>& g, const RnBwdPlan
   a.ld_gate = ld32(g.ld_gate), a.ld_stats = ld32(g.ld_stats), a.ld_dgate = ld32(g.ld_dgate);
   a.ld_dbranch = ld32(g.ld_dbranch), a.ld_dresidual = ld32(g.ld_dresidual);
   a.cols_per_gate = static_cast<unsigned>(g.cols_per_gate), a.cols_per_range = static_cast<unsigned>(g.cols_per_range);
+  a.ranges_per_gate = static_cast<unsigned>(g.ranges_per_gate);
   a.drop = g.drop, a.teams = plan.shape.row_teams(plan.teams);
   for (int q = 0; q < kGrads; ++q) a.part[q] = g.part[q];
   const unsigned lds = plan.teams > 1 ? static_cast<unsigned>(kMergeRows * plan.threads() * 8 * sizeof(float)) : 0;
@@ -324,11 +350,12 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   if (plan.shape.v) {
     const bool bias = dweights[kGradOutputBias] || dweights[kGradBranchBias] || (dgate && a.branch_bias);
     kernel = rn_bwd_kernel<T>(a, plan.shape, bias);
-    if (plan.twice && resident_blocks(kernel, plan.threads()) < 2 * kRnRanges) plan.cut(a.width, kRnRanges);
+    if (plan.twice && resident_blocks(kernel, plan.threads()) < 2 * kRnRanges)
+      plan.cut(a.width, dgate ? num_gates : 0, kRnRanges);
   }
   char* ws = static_cast<char*>(workspace);
   a.sums = reinterpret_cast<float*>(ws);
-  a.cols_per_range = plan.cols_per_range;
+  a.cols_per_range = plan.cols_per_range, a.ranges_per_gate = plan.ranges_per_gate;
   a.dgate = dgate, a.ld_dgate = ld_dgate;
   float* weights = reinterpret_cast<float*>(ws + plan.sums_bytes);
   RnMergeArgs merge{};
@@ -336,11 +363,14 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
     a.part[q] = !dweights[q] ? nullptr : plan.ranges == 1 ? dweights[q] : weights + q * plan.ranges * a.n;
     merge.part[q] = a.part[q], merge.out[q] = dweights[q];
   }
-  a.part[kGradGate] = dgate ? reinterpret_cast<float*>(ws + plan.sums_bytes + plan.weight_bytes) : nullptr;
-  merge.part[kGradGate] = a.part[kGradGate], merge.out[kGradGate] = dgate;
-  merge.n = a.n, merge.ranges = plan.ranges, merge.ld_dgate = ld_dgate, merge.num_gates = dgate ? num_gates : 0;
-  merge.cols_per_gate = a.cols_per_gate, merge.cols_per_range = plan.cols_per_range;
-  const int64_t items = kGradGate + merge.num_gates;
+  if (dgate && plan.ranges_per_gate) {
+    a.part[kGradGate] = reinterpret_cast<float*>(ws + plan.sums_bytes + plan.weight_bytes);
+    merge.part[kGradGate] = a.part[kGradGate], merge.out[kGradGate] = dgate;
+  }
+  merge.n = a.n, merge.ld_dgate = ld_dgate, merge.ranges = static_cast<unsigned>(plan.ranges);
+  merge.num_gates = merge.out[kGradGate] ? static_cast<unsigned>(num_gates) : 0;
+  merge.ranges_per_gate = static_cast<unsigned>(plan.ranges_per_gate);
+  const int64_t items = kGradGate + int64_t(merge.num_gates);
   auto capped = [](int64_t blocks) { return static_cast<unsigned>(blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30)); };
   const dim3 merge_grid(capped(ceil_div(a.n, 4 * kMergeLanes)), static_cast<unsigned>(items < 32768 ? items : 32768));
 
@@ -355,7 +385,8 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
                          dim3(256), 0, st, a);
     hipLaunchKernelGGL((rn_bwd_long_apply<T>), dim3(capped(ceil_div(a.n, 2048) * a.width)), dim3(256), 0, st, a);
   }
-  if ((weight_grads || dgate) && plan.ranges > 1)  // one range has written the gradients themselves
+  // one range has written the gradients themselves
+  if ((weight_grads && plan.ranges > 1) || merge.out[kGradGate])
     hipLaunchKernelGGL(rn_merge, merge_grid, dim3(kMergeLanes * kMergeGroups), 0, st, merge);
   return launch_status();
 }

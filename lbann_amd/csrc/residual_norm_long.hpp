@@ -41,8 +41,7 @@ struct RnFwdArgs {
   DropArgs drop;
 };
 
-// Partial gradients: row `slot` of quantity q at part[(q * slots + slot) * n]; the gate's rows
-// follow behind the last quantity.
+// Partial gradients: row b of part[q] is the sum over range b of the columns.
 enum RnGrad { kGradOutputScale = 0, kGradOutputBias, kGradBranchScale, kGradBranchBias, kGradGate, kGrads };
 
 template <typename T>
@@ -68,13 +67,30 @@ struct RnBwdArgs {
   T* dresidual;  // null: not wanted
   int64_t ld_dresidual;
   DropArgs drop;
-  // partial gradients of ranges of columns; part[q] null: not wanted
+  // partial gradients of ranges of columns; part[q] null: not wanted, or dgate written at once
   float* part[kGrads];
-  float* dgate;           // written at once for a gate whose columns all lie in one range
+  float* dgate;
   int64_t ld_dgate;
   float* sums;            // long kernels: four means per column
-  int64_t cols_per_range;
+  int64_t cols_per_range, ranges_per_gate;
 };
+
+// The columns of range b.  With ranges_per_gate > 0 no range reaches over the end of a gate's columns, each
+// leaves one partial row of the gate's gradient; with 0, all columns of a gate lie in one range (or
+// there is no gate), which writes the gate's gradient itself.
+template <typename I>
+__device__ __forceinline__ void rn_range(I b, I width, I cols_per_range, I cols_per_gate, I ranges_per_gate, I& first, I& last)
+{
+  if (ranges_per_gate) {
+    const I gate = b / ranges_per_gate;
+    first = gate * cols_per_gate + (b - gate * ranges_per_gate) * cols_per_range;
+    last = min(first + cols_per_range, (gate + 1) * cols_per_gate);
+  }
+  else {
+    first = b * cols_per_range;
+    last = min(first + cols_per_range, width);
+  }
+}
 
 // 1 / sqrt(v): 0 for an infinite variance and infinite for a zero one, as the formula has it
 // (the Newton step alone would turn both into NaN).
@@ -356,8 +372,8 @@ rn_bwd_long_columns(RnBwdArgs<T> a)
   const int64_t k = 8 * group, valid = a.n - k;
   if (valid <= 0) return;
   const int64_t range = blockIdx.y;
-  const int64_t first = range * a.cols_per_range;
-  const int64_t last = imin64(first + a.cols_per_range, a.width);
+  int64_t first, last;
+  rn_range<int64_t>(range, a.width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
   float acc[kGrads][8] = {};
   for (int64_t col = first; col < last; ++col) {
     const RnColumnStats s = rn_column_stats(a, col);
@@ -373,18 +389,14 @@ rn_bwd_long_columns(RnBwdArgs<T> a)
       acc[kGradBranchBias][j] += du[j];
       acc[kGradGate][j] += ev[j];
     }
-    if (a.part[kGradGate]) {
-      const int64_t gate = col / a.cols_per_gate;
-      if (col + 1 == last || (col + 1) / a.cols_per_gate != gate) {
-        const bool whole = first <= gate * a.cols_per_gate && (gate + 1) * a.cols_per_gate <= last;
-        store8((whole ? a.dgate + gate * a.ld_dgate : a.part[kGradGate] + (range + gate) * a.n) + k, valid, acc[kGradGate]);
+    if (a.dgate && a.ranges_per_gate == 0 && (col + 1) % a.cols_per_gate == 0) {
+      store8(a.dgate + col / a.cols_per_gate * a.ld_dgate + k, valid, acc[kGradGate]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
-      }
+      for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
     }
   }
 #pragma unroll
-  for (int q = 0; q < kGradGate; ++q)
+  for (int q = 0; q < kGrads; ++q)
     if (a.part[q]) store8(a.part[q] + range * a.n + k, valid, acc[q]);
 }
 

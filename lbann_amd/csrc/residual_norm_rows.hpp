@@ -285,7 +285,7 @@ struct RnBwdRows {
   const T *branch, *h, *dy, *dh;
   const float *gate, *branch_scale, *branch_bias, *output_scale, *stats;
   T *dbranch, *dresidual;
-  unsigned ld_branch, ld_h, ld_dy, ld_dh, ld_gate, ld_stats, ld_dbranch, ld_dresidual, ld_dgate, cols_per_gate, cols_per_range;
+  unsigned ld_branch, ld_h, ld_dy, ld_dh, ld_gate, ld_stats, ld_dbranch, ld_dresidual, ld_dgate, cols_per_gate, cols_per_range, ranges_per_gate;
   DropArgs drop;
   float* part[kGrads];
   float* dgate;
@@ -451,7 +451,7 @@ rn_bwd_rows(RnBwdRows<T> a)
   using U = Unit<T>;
   constexpr bool SUB = TEAM == 16;
   constexpr bool kKeepWeights = TEAM <= 512 || (!GATE && (sizeof(T) == 2 ? !(BRANCH_NORM && BIAS) : !BRANCH_NORM));
-  extern __shared__ float merged[];  // kMergeRows x blockDim x 8 floats if there are several teams
+  extern __shared__ __align__(16) float merged[];  // kMergeRows x blockDim x 8 floats if there are several teams
   __shared__ float* merged_rows[kMergeRows];
   __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
@@ -466,8 +466,8 @@ rn_bwd_rows(RnBwdRows<T> a)
   const bool several_gates = GATE && a.cols_per_gate < width;
   const bool output_norm = a.output_norm != kNormNone;
   const bool read_branch = BRANCH_NORM || (GATE && a.branch);
-  const unsigned first = blockIdx.x * a.cols_per_range;
-  const unsigned last = min(first + a.cols_per_range, width);
+  unsigned first, last;
+  rn_range(blockIdx.x, width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
 
   auto weights = [&](const float* w, float fill, float (&out)[8]) { share.weights(w, 0, fill, out); };
   float w2[8], w1[8], b1[8], gt[8];
@@ -502,8 +502,8 @@ rn_bwd_rows(RnBwdRows<T> a)
     }
   };
   // The sums of the quantities from FIRST to LAST whose row is given, over all teams: one row each.
-  // Several teams meet in LDS, kMergeRows rows at a time and by one piece of code for all rows (a copy
-  // of it for every quantity cost 2 us each on short ranges, in barriers and instruction fetches).
+  // Several teams meet in LDS, kMergeRows rows at a time, in 16-byte pieces and by one piece of code for
+  // all rows (one row after the other in single floats cost 1.5 us a row on short ranges).
   auto flush = [&](auto first_q, auto last_q, float* const (&rows)[kGrads]) {
     constexpr int kFirst = decltype(first_q)::value, kLast = decltype(last_q)::value;
     if (teams == 1) {
@@ -512,42 +512,43 @@ rn_bwd_rows(RnBwdRows<T> a)
         if (rows[q]) store_unit<EVEN>(rows[q] + entry, valid, acc[q]);
     }
     else {
-      const int stride = 8 * lanes;
+      const int stride = 8 * lanes, quads = (n + 3) / 4;
       auto round = [&](auto from_q, auto to_q) {
         int count = 0;
         __syncthreads();  // what was here has been read
 #pragma unroll
         for (int q = decltype(from_q)::value; q <= decltype(to_q)::value; ++q) {
           if (rows[q]) {
-            float* mine = merged + (count * teams + team.index) * stride + 8 * team.t;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mine[j] = acc[q][j];
+            v4f* mine = reinterpret_cast<v4f*>(merged + (count * teams + team.index) * stride + 8 * team.t);
+            mine[0] = v4f{acc[q][0], acc[q][1], acc[q][2], acc[q][3]};
+            mine[1] = v4f{acc[q][4], acc[q][5], acc[q][6], acc[q][7]};
             if (threadIdx.x == 0) merged_rows[count] = rows[q];
             ++count;
           }
         }
         __syncthreads();
-        for (int row = 0; row < count; ++row) {
-          float* out = merged_rows[row];
-          for (int k = threadIdx.x; k < n; k += static_cast<int>(blockDim.x)) {
-            float sum = 0.f;
-#pragma unroll 1
-            for (int i = 0; i < teams; ++i) sum += merged[(row * teams + i) * stride + k];
-            out[k] = sum;
+        for (int i = threadIdx.x; i < count * quads; i += static_cast<int>(blockDim.x)) {
+          const int row = (i >= quads) + (i >= 2 * quads), k = 4 * (i - row * quads);
+          const float* from = merged + row * teams * stride + k;
+          v4f sum = *reinterpret_cast<const v4f*>(from);
+#pragma unroll 3
+          for (int j = 1; j < teams; ++j) sum += *reinterpret_cast<const v4f*>(from + j * stride);
+          float* out = merged_rows[row] + k;
+          if (EVEN || k + 4 <= n) {
+            __builtin_memcpy(out, &sum, sizeof(sum));
+          }
+          else {
+#pragma unroll
+            for (int j = 0; j < 3; ++j)
+              if (k + j < n) out[j] = sum[j];
           }
         }
       };
+      static_assert(kMergeRows == 3, "the row of a piece is found by two comparisons");
       constexpr int kMid = kFirst + kMergeRows - 1 < kLast ? kFirst + kMergeRows - 1 : kLast;
       round(std::integral_constant<int, kFirst>{}, std::integral_constant<int, kMid>{});
       if constexpr (kMid < kLast) round(std::integral_constant<int, kMid + 1>{}, std::integral_constant<int, kLast>{});
     }
-  };
-  auto flush_gate = [&](unsigned gate, bool whole) {
-    float* rows[kGrads] = {};
-    rows[kGradGate] = whole ? column(a.dgate, gate, a.ld_dgate) : column(a.part[kGradGate], blockIdx.x + gate, n);
-    flush(std::integral_constant<int, kGradGate>{}, std::integral_constant<int, kGradGate>{}, rows);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
   };
 
   bool in_flight = false;
@@ -657,18 +658,22 @@ rn_bwd_rows(RnBwdRows<T> a)
       }
       if (active) store_unit<EVEN>(column(a.dbranch, col, a.ld_dbranch) + entry, valid, e);
     }
-    if (GATE && a.part[kGradGate] && several_gates)
-      flush_gate(gate, begin == gate * a.cols_per_gate && end == (gate + 1) * a.cols_per_gate);
+    if (GATE && a.dgate && a.ranges_per_gate == 0) {  // the gate's columns are all here
+      float* rows[kGrads] = {};
+      rows[kGradGate] = column(a.dgate, gate, a.ld_dgate);
+      flush(std::integral_constant<int, kGradGate>{}, std::integral_constant<int, kGradGate>{}, rows);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
+    }
     begin = end;
   }
   float* rows[kGrads];
 #pragma unroll
   for (int q = 0; q < kGrads; ++q) {
     const bool here = q == kGradOutputScale || (q == kGradOutputBias && BIAS) || (q == kGradBranchScale && BRANCH_NORM) ||
-                      (q == kGradBranchBias && BRANCH_NORM && BIAS) || (q == kGradGate && GATE && !several_gates);
+                      (q == kGradBranchBias && BRANCH_NORM && BIAS) || (q == kGradGate && GATE);
     rows[q] = here && a.part[q] ? column(a.part[q], blockIdx.x, n) : nullptr;
   }
-  if (GATE && !several_gates && a.part[kGradGate] && gridDim.x == 1) rows[kGradGate] = a.dgate;  // the only range
   flush(std::integral_constant<int, 0>{}, std::integral_constant<int, kGradGate>{}, rows);
 }
 
