@@ -927,6 +927,7 @@ class residual_norm_layer(_Dropout):
     and leaves the weights' gradients in m_{branch,output}_{scale,bias}_gradient and
     m_gate_gradient."""
 
+    _gradients = [(name, f"m_{name}_gradient") for name in ("branch_scale", "branch_bias", "output_scale", "output_bias")]
     KINDS = {"none": capi.LBN_NORM_NONE, "rms": capi.LBN_NORM_RMS, "layer": capi.LBN_NORM_LAYER}
 
     def __init__(self, size, branch_norm="none", output_norm="rms", epsilon=1e-5, residual_multiplier=1.0,
@@ -956,9 +957,9 @@ class residual_norm_layer(_Dropout):
                     raise ValueError(f"{name} has shape {tuple(t.shape)}; expected ({self.size},)")
         self.branch = self.h = self.gate = self.residual = self.activations = self.m_statistics = None
         self.m_has_residual = False
-        self.m_gate_gradient = None
-        for name in self.weights:
-            setattr(self, f"m_{name}_gradient", None)
+        self.m_gate_gradient = self._scratch_for = None
+        for _, attribute in self._gradients:
+            setattr(self, attribute, None)
 
     def _check_gate(self, gate, like):
         if gate is None:
@@ -1014,13 +1015,21 @@ class residual_norm_layer(_Dropout):
         dbranch = _matrix_beside(like, n, w)
         dres = _matrix_beside(like, n, w) if self.m_has_residual else None
         grads = []
-        for name in ("branch_scale", "branch_bias", "output_scale", "output_bias"):
-            g = None if wt[name] is None else _Vector(n, like.tensor.device)
-            setattr(self, f"m_{name}_gradient", g)
+        for name, attribute in self._gradients:
+            g = None
+            if wt[name] is not None:
+                g = _Vector.__new__(_Vector)
+                g.n, g.tensor = n, like.tensor.new_empty((n,), dtype=torch.float32)
+            setattr(self, attribute, g)
             grads.append(None if g is None else g.tensor.data_ptr())
         gates = 0 if gate is None else gate.width
         self.m_gate_gradient = dgate = None if gate is None else _matrix_beside(like, n, gates, torch.float32)
-        need = capi.lib().lbn_residual_norm_bwd_workspace_bytes(n, w, int(any(grads)), gates, like.tensor.element_size())
+        key = w, gates, like.tensor.dtype
+        if self._scratch_for != key:
+            self._scratch_for = key
+            self._scratch_bytes = capi.lib().lbn_residual_norm_bwd_workspace_bytes(
+                n, w, int(any(t is not None for t in wt.values())), gates, like.tensor.element_size())
+        need = self._scratch_bytes
         # scratch of this call alone: nothing that another stream or a recorded graph could share
         ws = like.tensor.new_empty((need,), dtype=torch.uint8) if need else None
         _entry("lbn_residual_norm_bwd", like.tensor.dtype)(
