@@ -380,10 +380,9 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   }
   else {
     hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(capped(a.width)), dim3(kRnLongThreads), 0, st, a);
-    if (weight_grads || dgate)
-      hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(capped(ceil_div(a.n, 2048)), static_cast<unsigned>(plan.ranges)),
-                         dim3(256), 0, st, a);
-    hipLaunchKernelGGL((rn_bwd_long_apply<T>), dim3(capped(ceil_div(a.n, 2048) * a.width)), dim3(256), 0, st, a);
+    const int64_t slices = ceil_div(a.n, 8 * kRnColumnThreads);
+    hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(capped(slices), static_cast<unsigned>(plan.ranges < 32768 ? plan.ranges : 32768)),
+                       dim3(kRnColumnThreads), 0, st, a, plan.ranges);
   }
   // one range has written the gradients themselves
   if ((weight_grads && plan.ranges > 1) || merge.out[kGradGate])

@@ -5,10 +5,10 @@
 // Forward: one workgroup per column; the moments of the block's output, then those of the new
 // residual stream, then both outputs, re-reading the column (from the caches) each time.
 // Backward: (1) one workgroup per column forms the up to four row means the gradients need
-// and leaves them in the workspace; (2) threads that own eight features walk a range of
-// columns and leave partial sums of the weight and gate gradients; (3) those are merged in a fixed
-// order (residual_norm.hip); (4) an entry-wise kernel writes the two gradients of the
-// activations.  (4) comes last because its outputs may take the place of its inputs.
+// and leaves them in the workspace; (2) threads that own eight features walk a range of columns,
+// write the gradients of the activations and leave partial sums of the weight and gate gradients;
+// (3) those are merged in a fixed order (residual_norm.hpp).  A thread of (2) writes what it alone
+// has read, so outputs may take the place of inputs.
 #pragma once
 
 #include "device_utils.hpp"
@@ -362,74 +362,57 @@ rn_bwd_long_sums(RnBwdArgs<T> a)
   }
 }
 
-// (2) Partial gradients: blockIdx.y is a range of columns, blockIdx.x a slice of features.
+// (2) Gradients of the activations and partial sums: blockIdx.x is a slice of features, blockIdx.y a
+// range of columns.
+constexpr int kRnColumnThreads = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(256)
-rn_bwd_long_columns(RnBwdArgs<T> a)
+__global__ void __launch_bounds__(kRnColumnThreads)
+rn_bwd_long_columns(RnBwdArgs<T> a, int64_t ranges)
 {
   const DropStream stream = drop_stream(a.drop);
-  const int64_t group = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t group = static_cast<int64_t>(blockIdx.x) * kRnColumnThreads + threadIdx.x;
   const int64_t k = 8 * group, valid = a.n - k;
   if (valid <= 0) return;
-  const int64_t range = blockIdx.y;
-  int64_t first, last;
-  rn_range<int64_t>(range, a.width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
-  float acc[kGrads][8] = {};
-  for (int64_t col = first; col < last; ++col) {
-    const RnColumnStats s = rn_column_stats(a, col);
-    const float* m = a.sums + 4 * col;
-    float e[8], dy[8], xh[8], du[8], uh[8], ev[8];
-    rn_stream_grad8(a, s, col, k, valid, m[0], m[1], e, dy, xh);
-    rn_branch_grad8(a, stream, s, col, k, valid, e, du, uh, ev);
+  for (int64_t range = blockIdx.y; range < ranges; range += gridDim.y) {
+    int64_t first, last;
+    rn_range<int64_t>(range, a.width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
+    float acc[kGrads][8] = {};
+    for (int64_t col = first; col < last; ++col) {
+      const RnColumnStats s = rn_column_stats(a, col);
+      const float* m = a.sums + 4 * col;
+      float e[8], dy[8], xh[8], du[8], uh[8], ev[8];
+      rn_stream_grad8(a, s, col, k, valid, m[0], m[1], e, dy, xh);
+      rn_branch_grad8(a, stream, s, col, k, valid, e, du, uh, ev);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      acc[kGradOutputScale][j] = __builtin_fmaf(dy[j], xh[j], acc[kGradOutputScale][j]);
-      acc[kGradOutputBias][j] += dy[j];
-      acc[kGradBranchScale][j] = __builtin_fmaf(du[j], uh[j], acc[kGradBranchScale][j]);
-      acc[kGradBranchBias][j] += du[j];
-      acc[kGradGate][j] += ev[j];
+      for (int j = 0; j < 8; ++j) {
+        acc[kGradOutputScale][j] = __builtin_fmaf(dy[j], xh[j], acc[kGradOutputScale][j]);
+        acc[kGradOutputBias][j] += dy[j];
+        acc[kGradBranchScale][j] = __builtin_fmaf(du[j], uh[j], acc[kGradBranchScale][j]);
+        acc[kGradBranchBias][j] += du[j];
+        acc[kGradGate][j] += ev[j];
+      }
+      if (a.dresidual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] *= a.residual_mult;
+        store8(a.dresidual + col * a.ld_dresidual + k, valid, e);
+      }
+      if (a.branch_norm != kNormNone) {
+        float w[8];
+        load_weights8(a.branch_scale, k, valid, 1.f, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) du[j] = s.rstd1 * (du[j] * w[j] - m[2] - uh[j] * m[3]);
+      }
+      store8(a.dbranch + col * a.ld_dbranch + k, valid, du);
+      if (a.dgate && a.ranges_per_gate == 0 && (col + 1) % a.cols_per_gate == 0) {
+        store8(a.dgate + col / a.cols_per_gate * a.ld_dgate + k, valid, acc[kGradGate]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
+      }
     }
-    if (a.dgate && a.ranges_per_gate == 0 && (col + 1) % a.cols_per_gate == 0) {
-      store8(a.dgate + col / a.cols_per_gate * a.ld_dgate + k, valid, acc[kGradGate]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < kGrads; ++q)
-    if (a.part[q]) store8(a.part[q] + range * a.n + k, valid, acc[q]);
-}
-
-// (4) The gradients of the activations.
-template <typename T>
-__global__ void __launch_bounds__(256)
-rn_bwd_long_apply(RnBwdArgs<T> a)
-{
-  const DropStream stream = drop_stream(a.drop);
-  const int64_t groups = (a.n + 7) / 8;
-  const int64_t tiles = (groups + 255) / 256;
-  for (int64_t item = blockIdx.x; item < tiles * a.width; item += gridDim.x) {
-    const int64_t col = item / tiles;
-    const int64_t group = (item - col * tiles) * 256 + threadIdx.x;
-    const int64_t k = 8 * group, valid = a.n - k;
-    if (valid <= 0) continue;
-    const RnColumnStats s = rn_column_stats(a, col);
-    const float* m = a.sums + 4 * col;
-    float e[8], dy[8], xh[8], du[8], uh[8], ev[8];
-    rn_stream_grad8(a, s, col, k, valid, m[0], m[1], e, dy, xh);
-    rn_branch_grad8(a, stream, s, col, k, valid, e, du, uh, ev);
-    if (a.branch_norm != kNormNone) {
-      float w[8];
-      load_weights8(a.branch_scale, k, valid, 1.f, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) du[j] = s.rstd1 * (du[j] * w[j] - m[2] - uh[j] * m[3]);
-    }
-    if (a.dresidual) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] *= a.residual_mult;
-      store8(a.dresidual + col * a.ld_dresidual + k, valid, e);
-    }
-    store8(a.dbranch + col * a.ld_dbranch + k, valid, du);
+    for (int q = 0; q < kGrads; ++q)
+      if (a.part[q]) store8(a.part[q] + range * a.n + k, valid, acc[q]);
   }
 }
 
