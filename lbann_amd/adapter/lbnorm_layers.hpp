@@ -11,7 +11,8 @@
 //   channelwise_softmax_layer   src/layers/misc/channelwise_softmax.cu
 // and, beyond those five, instance_norm_layer, entrywise_batch_normalization_layer,
 // cross_entropy_layer, entrywise_scale_bias_layer and channelwise_scale_bias_layer,
-// and gradient_buffer, where their weight gradients go (optimizer::add_to_gradient).
+// and gradient_buffer, where their weight gradients go (optimizer::add_to_gradient); and, for
+// transformers, dropout_layer, residual_norm_layer and logits_adjust_layer.
 //
 // `Mat` is any local-matrix type with the El::Matrix<T, El::Device::GPU> accessors
 //   Height(), Width(), LDim(), Buffer(), LockedBuffer()
@@ -1198,6 +1199,254 @@ public:
 private:
   device_matrix<float> m_gradient;
   optimizer_gradient_status m_status = optimizer_gradient_status::cleared;
+};
+
+
+// ------------------------------------------------- the residual stream and the logits
+/// Storage of bfloat16 entries for applications without a type of their own.
+struct bfloat16 {
+  uint16_t bits;
+};
+
+/// Which entry points serve an element type: float, or a 2-byte type holding IEEE binary16 unless
+/// this trait is specialised (as below) to say that it holds bfloat16.
+enum class storage { f32, f16, bf16 };
+template <typename T>
+struct storage_of {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 2, "fp32, fp16 or bfloat16 storage");
+  static constexpr storage value = sizeof(T) == 4 ? storage::f32 : storage::f16;
+};
+template <>
+struct storage_of<bfloat16> {
+  static constexpr storage value = storage::bf16;
+};
+
+/// Where the random bits of a layer come from (include/lbnorm.h, lbn_dropout_*).  Every
+/// training-mode forward takes the next offset; backward repeats the last one.
+struct dropout_state {
+  double keep_prob = 1.0;
+  uint64_t seed = 0, offset = 0, next_offset = 0;
+  int64_t column_offset = 0;       // global index of the first local column
+  const uint64_t* step = nullptr;  // device counter added to the offset (recorded graphs)
+  double kept = 1.0;               // keep probability of the last forward
+  void start(bool training)
+  {
+    if (training && keep_prob < 1.0) offset = next_offset++;
+    kept = training ? keep_prob : 1.0;
+  }
+};
+
+namespace detail {
+template <storage S, typename F32, typename F16, typename BF16>
+constexpr auto pick(F32 f32, F16 f16, BF16 bf16)
+{
+  if constexpr (S == storage::f32) return f32;
+  else if constexpr (S == storage::f16) return f16;
+  else return bf16;
+}
+/// Entry as the C ABI takes it: float*, or void* for the 2-byte types.
+template <typename T>
+using abi_t = std::conditional_t<storage_of<T>::value == storage::f32, float, void>;
+template <typename T, typename Mat>
+const abi_t<T>* in(const Mat* m) { return m ? reinterpret_cast<const abi_t<T>*>(m->LockedBuffer()) : nullptr; }
+template <typename T, typename Mat>
+abi_t<T>* out(Mat* m) { return m ? reinterpret_cast<abi_t<T>*>(m->Buffer()) : nullptr; }
+template <typename Mat>
+int64_t ld(const Mat* m) { return m ? m->LDim() : 0; }
+template <typename Mat>
+void require_shape(const Mat* m, int64_t h, int64_t w, const char* what)
+{
+  if (m && (m->Height() != h || m->Width() != w))
+    throw exception(std::string(what) + " is " + std::to_string(m->Height()) + " x " + std::to_string(m->Width()) +
+                    "; expected " + std::to_string(h) + " x " + std::to_string(w));
+}
+}  // namespace detail
+
+/// LBANN's dropout layer (include/lbann/layers/regularizers/dropout.hpp) with a mask that is formed
+/// from a counter in both directions and never stored.
+template <typename T = float, typename Mat = device_matrix<T>>
+class dropout_layer {
+public:
+  explicit dropout_layer(double keep_prob = 0.5, uint64_t seed = 0)
+  {
+    if (!(keep_prob > 0.0 && keep_prob <= 1.0)) throw exception("dropout keep probability must be in (0, 1]");
+    state.keep_prob = state.kept = keep_prob;
+    state.seed = seed;
+  }
+  layer_io<Mat> io;
+  dropout_state state;
+  bool is_training = true;
+
+  void fp_compute()
+  {
+    state.start(is_training);
+    run(detail::pick<storage_of<T>::value>(lbn_dropout_fwd_f32, lbn_dropout_fwd_f16, lbn_dropout_fwd_bf16),
+        *io.prev_activations, *io.activations, "dropout_layer::fp_compute");
+  }
+  void bp_compute()
+  {
+    run(detail::pick<storage_of<T>::value>(lbn_dropout_bwd_f32, lbn_dropout_bwd_f16, lbn_dropout_bwd_bf16),
+        *io.prev_error_signals, *io.error_signals, "dropout_layer::bp_compute");
+  }
+
+private:
+  template <typename F>
+  void run(F entry, const Mat& x, Mat& y, const char* where)
+  {
+    detail::require_shape(&y, x.Height(), x.Width(), where);
+    check_status(entry(io.stream, x.Height(), x.Width(), state.kept, state.seed, state.offset, state.step,
+                       state.column_offset, detail::in<T>(&x), x.LDim(), detail::out<T>(&y), y.LDim()), where);
+  }
+};
+
+/// The residual stream between two transformer blocks: u = N1(branch), v = dropout(u),
+/// h = a residual + b gate v, y = N2(h) (include/lbnorm.h, lbn_residual_norm_*).
+template <typename T = float, typename Mat = device_matrix<T>, typename Mat32 = device_matrix<float>>
+class residual_norm_layer {
+public:
+  residual_norm_layer(int branch_norm = LBN_NORM_NONE, int output_norm = LBN_NORM_RMS, double epsilon = 1e-5,
+                      double residual_multiplier = 1.0, double branch_multiplier = 1.0)
+    : m_branch_norm(branch_norm), m_output_norm(output_norm), m_epsilon(static_cast<float>(epsilon)),
+      m_a(static_cast<float>(residual_multiplier)), m_b(static_cast<float>(branch_multiplier))
+  {
+    for (int kind : {branch_norm, output_norm})
+      if (kind < LBN_NORM_NONE || kind > LBN_NORM_LAYER) throw exception("residual_norm_layer: unknown norm kind");
+  }
+  /// Weight vectors of the two norms (device memory, NULL for 1 resp. 0) and their gradients (NULL: not wanted).
+  void set_weights(const float* branch_scale, const float* branch_bias, const float* output_scale, const float* output_bias)
+  {
+    m_w[0] = branch_scale, m_w[1] = branch_bias, m_w[2] = output_scale, m_w[3] = output_bias;
+  }
+  void set_weight_gradients(float* dbranch_scale, float* dbranch_bias, float* doutput_scale, float* doutput_bias)
+  {
+    m_g[0] = dbranch_scale, m_g[1] = dbranch_bias, m_g[2] = doutput_scale, m_g[3] = doutput_bias;
+  }
+
+  hipStream_t stream = nullptr;
+  const Mat* branch = nullptr;          // the block's output
+  const Mat* residual = nullptr;        // the stream before it (may stay null)
+  const Mat32* gate = nullptr;          // one column per width / gate->Width() columns (may stay null)
+  Mat* new_residual = nullptr;          // h; backward reads it
+  Mat* output = nullptr;                // y; null without an output norm
+  const Mat* output_gradient = nullptr;        // dL/dy; null without an output norm
+  const Mat* new_residual_gradient = nullptr;  // dL/dh apart from y's part (may stay null with an output norm)
+  Mat* branch_gradient = nullptr;
+  Mat* residual_gradient = nullptr;     // may stay null
+  Mat32* gate_gradient = nullptr;       // may stay null
+  dropout_state state;
+  bool is_training = true;
+  device_matrix<float> m_statistics;    // 4 x width, written in training mode
+
+  void fp_compute()
+  {
+    const char* where = "residual_norm_layer::fp_compute";
+    if (!branch) throw exception("residual_norm_layer::fp_compute: no branch");
+    const int64_t n = branch->Height(), w = branch->Width();
+    detail::require_shape(residual, n, w, "residual");
+    detail::require_shape(new_residual, n, w, "new_residual");
+    detail::require_shape(output, n, w, "output");
+    check_gate(n, w);
+    state.start(is_training);
+    if (is_training) m_statistics.Resize(4, w);
+    const auto entry = detail::pick<storage_of<T>::value>(lbn_residual_norm_fwd_f32, lbn_residual_norm_fwd_f16,
+                                                          lbn_residual_norm_fwd_bf16);
+    check_status(entry(stream, n, w, m_branch_norm, m_output_norm, m_epsilon, m_a, m_b, detail::in<T>(branch),
+                       branch->LDim(), detail::in<T>(residual), detail::ld(residual), gate_buffer(), detail::ld(gate),
+                       gates(), m_w[0], m_w[1], m_w[2], m_w[3], state.kept, state.seed, state.offset, state.step,
+                       state.column_offset, detail::out<T>(new_residual), detail::ld(new_residual), detail::out<T>(output),
+                       detail::ld(output), is_training ? m_statistics.Buffer() : nullptr, m_statistics.LDim()),
+                 where);
+  }
+
+  void bp_compute()
+  {
+    const char* where = "residual_norm_layer::bp_compute";
+    const Mat* like = output_gradient ? output_gradient : new_residual_gradient;
+    if (!like) throw exception("residual_norm_layer::bp_compute: no gradient");
+    const int64_t n = like->Height(), w = like->Width();
+    for (const Mat* m : {branch, static_cast<const Mat*>(new_residual), output_gradient, new_residual_gradient,
+                         static_cast<const Mat*>(branch_gradient), static_cast<const Mat*>(residual_gradient)})
+      detail::require_shape(m, n, w, where);
+    check_gate(n, w);
+    detail::require_shape(gate_gradient, n, gates(), "gate_gradient");
+    if (m_statistics.Width() != w) throw exception("residual_norm_layer::bp_compute needs a training-mode forward first");
+    const bool weights = m_g[0] || m_g[1] || m_g[2] || m_g[3];
+    const size_t bytes = lbn_residual_norm_bwd_workspace_bytes(n, w, weights ? 1 : 0, gate_gradient ? gates() : 0,
+                                                               static_cast<int>(sizeof(T)));
+    void* ws = m_ws.reserve(bytes, stream);
+    const auto entry = detail::pick<storage_of<T>::value>(lbn_residual_norm_bwd_f32, lbn_residual_norm_bwd_f16,
+                                                          lbn_residual_norm_bwd_bf16);
+    const Mat* h = m_output_norm != LBN_NORM_NONE ? new_residual : nullptr;
+    check_status(entry(stream, n, w, m_branch_norm, m_output_norm, m_epsilon, m_a, m_b, detail::in<T>(branch),
+                       detail::ld(branch), detail::in<T>(h), detail::ld(h), gate_buffer(), detail::ld(gate), gates(),
+                       m_w[0], m_w[1], m_w[2], state.kept, state.seed, state.offset, state.step, state.column_offset,
+                       m_statistics.LockedBuffer(), m_statistics.LDim(), detail::in<T>(output_gradient),
+                       detail::ld(output_gradient), detail::in<T>(new_residual_gradient), detail::ld(new_residual_gradient),
+                       detail::out<T>(branch_gradient), detail::ld(branch_gradient), detail::out<T>(residual_gradient),
+                       detail::ld(residual_gradient), gate_gradient ? gate_gradient->Buffer() : nullptr,
+                       detail::ld(gate_gradient), m_g[0], m_g[1], m_g[2], m_g[3], ws, bytes),
+                 where);
+  }
+  /// Backward's scratch buffer (reserve it up front to keep the hook free of allocation).
+  workspace& scratch() { return m_ws; }
+
+private:
+  int64_t gates() const { return gate ? gate->Width() : 0; }
+  const float* gate_buffer() const { return gate ? gate->LockedBuffer() : nullptr; }
+  void check_gate(int64_t n, int64_t w) const
+  {
+    if (gate && (gate->Height() != n || gate->Width() < 1 || w % gate->Width() != 0))
+      throw exception("residual_norm_layer: the gate has the wrong height or a number of columns that does not divide the width");
+  }
+  int m_branch_norm, m_output_norm;
+  float m_epsilon, m_a, m_b;
+  const float* m_w[4] = {};
+  float* m_g[4] = {};
+  workspace m_ws;
+};
+
+/// Penalties for repeated tokens, bias lists and grammar masks on the logits of a decoding step
+/// (include/lbnorm.h, lbn_logits_adjust_*), before the softmax layer.
+template <typename T = float, typename Mat = device_matrix<T>, typename MatInt = device_matrix<int32_t>,
+          typename Mat32 = device_matrix<float>>
+class logits_adjust_layer {
+public:
+  hipStream_t stream = nullptr;
+  const Mat* logits = nullptr;      // vocabulary x sequences
+  Mat* output = nullptr;            // may be the same matrix
+  const MatInt* tokens = nullptr;   // max_tokens x sequences; everything from here on may stay null
+  const int32_t* lengths = nullptr;
+  const int32_t* prompt_lengths = nullptr;
+  const float* repetition = nullptr;
+  const float* presence = nullptr;
+  const float* frequency = nullptr;
+  const MatInt* bias_tokens = nullptr;  // entries x sequences
+  const Mat32* bias_values = nullptr;
+  const MatInt* mask = nullptr;         // 32-bit words x grammars
+  const int32_t* mask_index = nullptr;
+
+  void fp_compute()
+  {
+    const char* where = "logits_adjust_layer::fp_compute";
+    if (!logits || !output) throw exception("logits_adjust_layer::fp_compute: no logits or no output");
+    const int64_t v = logits->Height(), w = logits->Width();
+    detail::require_shape(output, v, w, "output");
+    if (tokens) detail::require_shape(tokens, tokens->Height(), w, "tokens");
+    if (!bias_tokens != !bias_values) throw exception("logits_adjust_layer: bias tokens and values go together");
+    const int64_t biases = bias_tokens ? bias_tokens->Height() : 0;
+    detail::require_shape(bias_tokens, biases, w, "bias_tokens");
+    detail::require_shape(bias_values, biases, w, "bias_values");
+    if (mask) detail::require_shape(mask, (v + 31) / 32, mask->Width(), "mask");
+    const auto entry = detail::pick<storage_of<T>::value>(lbn_logits_adjust_f32, lbn_logits_adjust_f16, lbn_logits_adjust_bf16);
+    check_status(entry(stream, v, w, detail::in<T>(logits), logits->LDim(), detail::out<T>(output), output->LDim(),
+                       tokens ? tokens->LockedBuffer() : nullptr, detail::ld(tokens), tokens ? tokens->Height() : 0,
+                       lengths, prompt_lengths, repetition, presence, frequency,
+                       bias_tokens ? bias_tokens->LockedBuffer() : nullptr, detail::ld(bias_tokens),
+                       bias_values ? bias_values->LockedBuffer() : nullptr, detail::ld(bias_values), biases,
+                       mask ? reinterpret_cast<const uint32_t*>(mask->LockedBuffer()) : nullptr, detail::ld(mask),
+                       mask ? mask->Width() : 0, mask_index),
+                 where);
+  }
 };
 
 }  // namespace lbnorm

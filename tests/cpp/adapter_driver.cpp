@@ -504,6 +504,98 @@ int drv_cluster_wait_check(int64_t h, int64_t w, float* x, float* y, float* out4
   }
 }
 
+}  // extern "C"
+
+// A step over the residual stream through the C++ classes: dropout on the stream, residual norm
+// forward and backward, logits adjustment of its output.  All matrices n x w with leading
+// dimension n; gate n x gates.
+template <typename T>
+static int run_stream(int64_t n, int64_t w, int64_t gates, int branch_norm, int output_norm, double keep, void* const* m,
+                      const float* gate, float* dgate, float* const* weights, float* const* grads, const int32_t* tokens,
+                      int64_t max_tokens, const float* repetition, void* stream)
+{
+  // m: residual, branch, dropped, h, y, dy, dh, dbranch, ddropped, dresidual, adjusted
+  device_matrix<T> x[11];
+  for (int i = 0; i < 11; ++i) attach(x[i], n, w, m[i], n);
+  device_matrix<float> mg, mdg;
+  attach(mg, n, gates, const_cast<float*>(gate), n);
+  attach(mdg, n, gates, dgate, n);
+  device_matrix<int32_t> tok;
+  attach(tok, max_tokens, w, const_cast<int32_t*>(tokens), max_tokens);
+  dropout_layer<T> drop(keep, 11);
+  drop.io.stream = static_cast<hipStream_t>(stream);
+  drop.io.prev_activations = &x[0]; drop.io.activations = &x[2];
+  drop.io.prev_error_signals = &x[8]; drop.io.error_signals = &x[9];
+  residual_norm_layer<T> layer(branch_norm, output_norm, 1e-5, 0.75, 1.25);
+  layer.stream = drop.io.stream;
+  layer.state.keep_prob = keep; layer.state.seed = 77; layer.state.next_offset = 5;
+  layer.set_weights(weights[0], weights[1], weights[2], weights[3]);
+  layer.set_weight_gradients(grads[0], grads[1], grads[2], grads[3]);
+  layer.branch = &x[1]; layer.residual = &x[2]; layer.gate = &mg; layer.new_residual = &x[3]; layer.output = &x[4];
+  layer.output_gradient = &x[5]; layer.new_residual_gradient = &x[6];
+  layer.branch_gradient = &x[7]; layer.residual_gradient = &x[8]; layer.gate_gradient = &mdg;
+  logits_adjust_layer<T> adjust;
+  adjust.stream = drop.io.stream;
+  adjust.logits = &x[4]; adjust.output = &x[10]; adjust.tokens = &tok; adjust.repetition = repetition;
+  drop.fp_compute();
+  layer.fp_compute();
+  layer.bp_compute();
+  drop.bp_compute();
+  adjust.fp_compute();
+  check_hip(hipStreamSynchronize(drop.io.stream), "sync");
+  return 0;
+}
+
+extern "C" {
+
+// type: 0 fp32, 1 binary16, 2 bfloat16
+int drv_stream(int type, int64_t n, int64_t w, int64_t gates, int branch_norm, int output_norm, double keep, void* const* m,
+               const float* gate, float* dgate, float* const* weights, float* const* grads, const int32_t* tokens,
+               int64_t max_tokens, const float* repetition, void* stream, char* err, int errlen)
+{
+  try {
+    if (type == 0)
+      return run_stream<float>(n, w, gates, branch_norm, output_norm, keep, m, gate, dgate, weights, grads, tokens, max_tokens,
+                               repetition, stream);
+    if (type == 1)
+      return run_stream<uint16_t>(n, w, gates, branch_norm, output_norm, keep, m, gate, dgate, weights, grads, tokens, max_tokens,
+                                  repetition, stream);
+    return run_stream<bfloat16>(n, w, gates, branch_norm, output_norm, keep, m, gate, dgate, weights, grads, tokens, max_tokens,
+                                repetition, stream);
+  }
+  catch (const std::exception& e) {
+    return fail(e, err, errlen);
+  }
+}
+
+// What the classes of the residual stream refuse, without touching a device.
+int drv_stream_error_cases(void)
+{
+  int missed = 0;
+  auto throws = [&](auto f) {
+    try { f(); ++missed; } catch (const exception&) {}
+  };
+  throws([] { dropout_layer<> l(0.0); });
+  throws([] { dropout_layer<> l(1.5); });
+  throws([] { residual_norm_layer<> l(3, 1); });
+  device_matrix<float> a, b, g;
+  a.Attach(8, 6, nullptr, 8); b.Attach(8, 5, nullptr, 8); g.Attach(8, 4, nullptr, 8);
+  throws([&] { residual_norm_layer<> l; l.fp_compute(); });
+  throws([&] { residual_norm_layer<> l; l.branch = &a; l.residual = &b; l.fp_compute(); });
+  throws([&] { residual_norm_layer<> l; l.branch = &a; l.gate = &g; l.fp_compute(); });          // 4 does not divide 6
+  throws([&] { residual_norm_layer<> l; l.is_training = false; l.branch = &a; l.fp_compute(); });  // buffers missing: refused by the ABI
+  throws([&] { residual_norm_layer<> l; l.bp_compute(); });
+  throws([&] { residual_norm_layer<> l; l.output_gradient = &a; l.bp_compute(); });              // no forward yet
+  throws([&] { logits_adjust_layer<> l; l.fp_compute(); });
+  throws([&] { logits_adjust_layer<> l; l.logits = &a; l.output = &b; l.fp_compute(); });
+  throws([&] { logits_adjust_layer<> l; l.logits = &a; l.output = &a; l.bias_values = &a; l.fp_compute(); });
+  dropout_state s;
+  s.keep_prob = 0.5;
+  s.start(true); s.start(true); s.start(false);
+  if (s.offset != 1 || s.kept != 1.0 || s.next_offset != 2) ++missed;
+  return missed;
+}
+
 int drv_error_cases(void)
 {
   int missed = 0;
