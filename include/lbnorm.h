@@ -770,7 +770,8 @@ int lbn_dropout_bwd_bf16(lbn_stream_t stream, int64_t height, int64_t width, dou
  *   squares; no norm: 0 and 1), kept for backward; NULL if not wanted (inference).
  * Outputs may take the place of inputs of the same shape and leading dimension (h that of r or
  * o, y likewise).  Storage fp32, IEEE binary16 or bfloat16; arithmetic, statistics, weights,
- * gates and their gradients fp32. */
+ * gates and their gradients fp32.  LBN_ERR_UNSUPPORTED beyond 2^26 features, or 2^32 columns
+ * (column_offset included). */
 #define LBN_NORM_NONE 0
 #define LBN_NORM_RMS 1
 #define LBN_NORM_LAYER 2
@@ -877,7 +878,8 @@ int lbn_residual_norm_bwd_bf16(lbn_stream_t stream, int64_t size, int64_t width,
  * A grammar that allows nothing leaves a column of -infinity, on which the softmax layers
  * return NaN: end such a sequence first.  x and y may be the same matrix.  No workspace.
  * Storage fp32, IEEE binary16 or bfloat16, fp32 arithmetic, one rounding.
- * LBN_ERR_UNSUPPORTED beyond some 2^31 entries, sequences or tokens, or where one 32-bit word
+ * LBN_ERR_UNSUPPORTED beyond some 2^31 entries or tokens or 2^23 sequences (fewer where the
+ * vocabulary takes several workgroups), or where one 32-bit word
  * cannot hold a count up to max_tokens, a place in the bias list and one bit more (131072 tokens
  * leave room for 8191 biases). */
 int lbn_logits_adjust_f32(lbn_stream_t stream, int64_t vocabulary, int64_t width, const float* x,

@@ -59,8 +59,7 @@ static int dropout_launch(lbn_stream_t stream, int64_t height, int64_t width, do
   int lanes = 1;
   while (lanes < groups && lanes < kDropThreads) lanes *= 2;
   const int64_t items = ceil_div(groups, lanes) * ceil_div(width, kDropThreads / lanes);
-  const unsigned grid = static_cast<unsigned>(items < (int64_t(1) << 30) ? items : (int64_t(1) << 30));
-  hipLaunchKernelGGL((dropout_apply<T>), dim3(grid), dim3(kDropThreads), 0, st, x, ldx, y, ldy, height, width, lanes,
+  hipLaunchKernelGGL((dropout_apply<T>), dim3(walking_grid(items)), dim3(kDropThreads), 0, st, x, ldx, y, ldy, height, width, lanes,
                      drop_args(keep_prob, seed, offset, step, column_offset));
   return launch_status();
 }

@@ -79,6 +79,14 @@ inline bool rows_aligned16(const void* base, int64_t stride, int64_t ld, int64_t
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Workgroups of a launch whose kernel walks on by gridDim: never so many that their threads pass
+// the 2^32 that a launch can have.
+inline unsigned walking_grid(int64_t blocks)
+{
+  constexpr int64_t most = int64_t(1) << 21;
+  return static_cast<unsigned>(blocks < most ? blocks : most);
+}
+
 // Shape of a register-resident row kernel: `tpr` threads own a row and each keeps
 // `v` 16-byte vectors of it in registers.  tpr == 0: the row does not fit.
 struct RowConfig {

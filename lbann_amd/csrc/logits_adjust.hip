@@ -203,7 +203,7 @@ static int logits_adjust(lbn_stream_t stream, LogitsArgs<T> a)
   if (a.num_biases >> (31 - a.count_bits)) return LBN_ERR_UNSUPPORTED;
   const LogitsShape shape = logits_shape(a.max_tokens);
   a.slabs = static_cast<unsigned>(ceil_div(a.vocabulary, shape.slab()));
-  if (a.slabs * a.width > limit) return LBN_ERR_UNSUPPORTED;
+  if (a.slabs * a.width * shape.threads > limit) return LBN_ERR_UNSUPPORTED;  // threads of a launch
   const dim3 grid(static_cast<unsigned>(a.slabs * a.width));
   const unsigned lds = static_cast<unsigned>(shape.slab() * sizeof(uint32_t));
   hipStream_t st = as_stream(stream);

@@ -112,6 +112,8 @@ struct RnShape {
 // matrices in turn; forward 256 MiB in 50.3 -> 44.6 us, 128 MiB in 23 -> 25 us).
 constexpr int64_t kRnStreamBytes = int64_t(256) << 20;
 
+constexpr int64_t kRnMostFeatures = int64_t(1) << 26;  // the merge of partial rows has a workgroup for 64 of them
+
 static unsigned ld32(int64_t ld) { return static_cast<unsigned>(ld); }
 
 // Leading dimensions (0 for a matrix that is not there) and widths that the row kernels' 32-bit indices hold.
@@ -262,7 +264,7 @@ static void rn_launch_fwd(hipStream_t st, const RnFwdArgs<T>& g, const RnShape& 
   const int64_t blocks = ceil_div(g.width, shape.teams());
   const int64_t resident = resident_blocks(rn_fwd_rows<T, V, SUB, EVEN, STREAM>, shape.threads());
   const int64_t grid = resident > 0 && blocks > resident ? resident : blocks;
-  hipLaunchKernelGGL((rn_fwd_rows<T, V, SUB, EVEN, STREAM>), dim3(static_cast<unsigned>(grid)), dim3(shape.threads()), 0, st, a);
+  hipLaunchKernelGGL((rn_fwd_rows<T, V, SUB, EVEN, STREAM>), dim3(walking_grid(grid)), dim3(shape.threads()), 0, st, a);
 }
 
 template <typename T, bool EVEN, bool STREAM>
@@ -291,7 +293,7 @@ static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double
       !rn_ld_ok(a.gate, a.ld_gate, a.n, num_gates) || !rn_ld_ok(a.h, a.ld_h, a.n, a.width) ||
       !rn_ld_ok(a.y, a.ld_y, a.n, a.width) || !rn_ld_ok(a.stats, a.ld_stats, 4, a.width))
     return LBN_ERR_INVALID_ARGUMENT;
-  if (!drop_range_ok(a.n, a.width, column_offset)) return LBN_ERR_UNSUPPORTED;
+  if (a.n > kRnMostFeatures || !drop_range_ok(a.n, a.width, column_offset)) return LBN_ERR_UNSUPPORTED;
   a.cols_per_gate = num_gates > 0 ? a.width / num_gates : a.width;
   a.drop = drop_args(keep_prob, seed, offset, step, column_offset);
   hipStream_t st = as_stream(stream);
@@ -304,8 +306,7 @@ static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double
     else rn_launch_fwd<T, true, false>(st, a, shape);
   }
   else {
-    const int64_t grid = a.width < (int64_t(1) << 30) ? a.width : (int64_t(1) << 30);
-    hipLaunchKernelGGL((rn_fwd_long<T>), dim3(static_cast<unsigned>(grid)), dim3(kRnLongThreads), 0, st, a);
+    hipLaunchKernelGGL((rn_fwd_long<T>), dim3(walking_grid(a.width)), dim3(kRnLongThreads), 0, st, a);
   }
   return launch_status();
 }
@@ -334,7 +335,7 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
       !rn_ld_ok(a.dh, a.ld_dh, a.n, a.width) || !rn_ld_ok(a.dbranch, a.ld_dbranch, a.n, a.width) ||
       !rn_ld_ok(a.dresidual, a.ld_dresidual, a.n, a.width))
     return LBN_ERR_INVALID_ARGUMENT;
-  if (!drop_range_ok(a.n, a.width, column_offset)) return LBN_ERR_UNSUPPORTED;
+  if (a.n > kRnMostFeatures || !drop_range_ok(a.n, a.width, column_offset)) return LBN_ERR_UNSUPPORTED;
   if (!norm1 && !dgate) a.branch = nullptr;  // not needed, so not read
   a.cols_per_gate = num_gates > 0 ? a.width / num_gates : a.width;
   a.drop = drop_args(keep_prob, seed, offset, step, column_offset);
@@ -371,17 +372,16 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   merge.num_gates = merge.out[kGradGate] ? static_cast<unsigned>(num_gates) : 0;
   merge.ranges_per_gate = static_cast<unsigned>(plan.ranges_per_gate);
   const int64_t items = kGradGate + int64_t(merge.num_gates);
-  auto capped = [](int64_t blocks) { return static_cast<unsigned>(blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30)); };
-  const dim3 merge_grid(capped(ceil_div(a.n, 4 * kMergeLanes)), static_cast<unsigned>(items < 32768 ? items : 32768));
+  const dim3 merge_grid(static_cast<unsigned>(ceil_div(a.n, 4 * kMergeLanes)), static_cast<unsigned>(items < 32768 ? items : 32768));
 
   hipStream_t st = as_stream(stream);
   if (plan.shape.v) {
     rn_launch_bwd<T>(st, a, plan, kernel);
   }
   else {
-    hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(capped(a.width)), dim3(kRnLongThreads), 0, st, a);
+    hipLaunchKernelGGL((rn_bwd_long_sums<T>), dim3(walking_grid(a.width)), dim3(kRnLongThreads), 0, st, a);
     const int64_t slices = ceil_div(a.n, 8 * kRnColumnThreads);
-    hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(capped(slices), static_cast<unsigned>(plan.ranges < 32768 ? plan.ranges : 32768)),
+    hipLaunchKernelGGL((rn_bwd_long_columns<T>), dim3(static_cast<unsigned>(slices), static_cast<unsigned>(plan.ranges < 32768 ? plan.ranges : 32768)),
                        dim3(kRnColumnThreads), 0, st, a, plan.ranges);
   }
   // one range has written the gradients themselves

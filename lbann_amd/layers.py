@@ -970,8 +970,8 @@ class residual_norm_layer(_Dropout):
                              f"{like.tensor.device} and a number of columns that divides {like.width}")
 
     def forward(self, branch, residual=None, gate=None, training=True, offset=None, in_place=False):
-        """in_place: the new stream overwrites `residual` and y overwrites `branch` (inference: backward
-        needs what they held).  training=False: no dropout, no statistics."""
+        """in_place: the new stream overwrites `residual`, and outside training, where no backward
+        needs it, y overwrites `branch`.  training=False: no dropout, no statistics."""
         n, w, kinds, wt = self.size, branch.width, self._kinds, self.weights
         _same_kind(branch, n, w, branch=branch, residual=residual)
         stream = _stream_for(branch)
@@ -981,7 +981,7 @@ class residual_norm_layer(_Dropout):
         h = residual if in_place and residual is not None else _matrix_beside(branch, n, w)
         y = None
         if kinds[1]:
-            y = branch if in_place else _matrix_beside(branch, n, w)
+            y = branch if in_place and not training else _matrix_beside(branch, n, w)
         self.m_statistics = _matrix_beside(branch, 4, w, torch.float32) if training else None
         _entry("lbn_residual_norm_fwd", branch.tensor.dtype)(
             stream, n, w, *kinds, self.m_epsilon, self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch),

@@ -360,7 +360,7 @@ def test_decoding_step(L):
     # 2^-11 (|z| + sum of |y w|) ~ 0.02), the probability itself by 2^-11: a factor of exp(2 * 0.02)
     assert (probs[np.isneginf(z)] == 0).all()
     near = e > 2.0 ** -13
-    assert near.sum() > 100 and np.abs(probs / e - 1)[near].max() < 0.05
+    assert near.sum() > 100 and np.abs(probs[near] / e[near] - 1).max() < 0.05
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = step()
@@ -464,6 +464,73 @@ def test_layers_refuse_another_place(L):
         L.logits_adjust_layer(8).forward(x, bias_tokens=L.DeviceMatrix(3, 2, dtype=torch.int32))
     with pytest.raises(ValueError):
         L.residual_norm_layer(8).forward(x, gate=L.DeviceMatrix(8, 3))
+
+
+def test_empty_calls(L):
+    """No columns, or no sequences: nothing happens, nothing fails."""
+    layer = L.residual_norm_layer(16, "rms", "rms", output_scale=np.ones(16))
+    none = L.DeviceMatrix(16, 0)
+    y = layer.forward(none, none, L.DeviceMatrix(16, 2))
+    assert (y.height, y.width) == (16, 0)
+    db, dr = layer.backward(none, none)
+    assert db.width == dr.width == 0
+    assert L.dropout_layer(0.5).forward(none).width == 0
+    assert L.logits_adjust_layer(16).forward(none, L.DeviceMatrix(0, 0, dtype=torch.int32)).width == 0
+    x = L.DeviceMatrix(16, 3, fill=2.0)
+    y = L.logits_adjust_layer(16).forward(x, L.DeviceMatrix.attach(torch.empty(3, 0, dtype=torch.int32, device="cuda"), 0))
+    assert (y.tensor == 2).all()
+
+
+def test_residual_norm_in_place_while_training(L):
+    """The new stream may take the old one's place in training too; the block's output is kept for backward."""
+    n, t = 640, 9
+    rng = np.random.default_rng(2)
+    p, layer, gate, gate_v, data = make(L, rng, n, t, ("layer", "rms", 3, 0.8, True), "bf16", 0, 0)
+    y = layer.forward(data["o"][0], data["r"][0], gate, offset=5, in_place=True)
+    assert layer.residual is data["r"][0] and y is not data["o"][0]
+    h, want, _, size_h, size_y = ref.forward(data["o"][1], data["r"][1], gate_v, p)
+    close("h", got(layer.residual), h, size_h, "bf16", ref.roundings(n))
+    close("y", got(y), want, size_y, "bf16", ref.roundings(n))
+    check_backward(layer, p, gate_v, data, "bf16", n, t)
+
+
+def test_many_short_columns(L):
+    """More columns than a launch has workgroups, fewer features than a whole unit."""
+    n, t = 3, (1 << 21) + 77
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    o, dy = (torch.randn(t, n, generator=gen, device="cuda") for _ in range(2))
+    A = L.DeviceMatrix.attach
+    layer = L.residual_norm_layer(n, "none", "layer", output_scale=np.ones(n))
+    y = layer.forward(A(o, n)).tensor.double()
+    c = o.double() - o.double().mean(1, keepdim=True)
+    rstd = (c.square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    assert ((y - c * rstd).abs() <= ref.roundings(n) * ref.U * ((o.abs().double() + o.abs().double().mean(1, keepdim=True)) * rstd + 2)).all()
+    db, _ = layer.backward(A(dy, n))
+    assert torch.isfinite(db.tensor).all()
+    want = (dy.double() * c * rstd).sum(0)
+    size = (dy.abs().double() * (o.abs().double() + o.abs().double().mean(1, keepdim=True)) * rstd).sum(0)
+    assert ((layer.m_output_scale_gradient.tensor.double() - want).abs() <= ref.roundings(n, t) * ref.U * size).all()
+    drop = L.dropout_layer(0.5, seed=8)
+    wide = torch.ones(t, 9, device="cuda", dtype=torch.bfloat16)
+    kept = drop.forward(A(wide, 9), offset=0).tensor[-50:] != 0
+    assert np.array_equal(kept.cpu().numpy(), ref.keep_mask(9, 50, 0.5, 8, 0, t - 50))
+
+
+@pytest.mark.parametrize("n", [64, 1000, 1024])
+def test_leading_dimensions_beyond_32_bits(L, n):
+    """Columns more than 2^31 entries apart give what neighbouring ones give, within rounding."""
+    far = torch.zeros((1 << 31) + 4096, dtype=torch.bfloat16, device="cuda")
+    t = far.as_strided((2, n), ((1 << 31) + 8, 1))
+    rng = np.random.default_rng(n)
+    p, layer, _, _, data = make(L, rng, n, 2, ("rms", "layer", 0, 0.9, True), "bf16", 0, 0)
+    t.copy_(data["o"][0].tensor)
+    o = L.DeviceMatrix.attach(t, n)
+    assert o.ldim == (1 << 31) + 8
+    out = layer.forward(o, data["r"][0], offset=5)
+    h, y, _, size_h, size_y = ref.forward(data["o"][1], data["r"][1], None, p)
+    close("h", got(layer.residual), h, size_h, "bf16", ref.roundings(n))
+    close("y", got(out), y, size_y, "bf16", ref.roundings(n))
+    check_backward(layer, p, None, data, "bf16", n, 2)
 
 
 def test_offsets_beyond_32_bits(L):

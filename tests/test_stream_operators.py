@@ -113,6 +113,8 @@ def test_residual_norm_forward_refusals(suffix):
                 dict(keep=0.0), dict(keep=float("nan")), dict(col=-1)):
         assert call(**bad) == INVALID, bad
     assert call(col=2 ** 32 - 5) == UNSUPPORTED
+    big = {k: 2 ** 26 + 1 for k in ("n", "ldo", "ldr", "ldg", "ldh", "ldy")}
+    assert call(**big) == UNSUPPORTED
 
 
 @pytest.mark.parametrize("suffix", ["f32", "f16", "bf16"])
@@ -150,6 +152,7 @@ def test_logits_adjust_refusals(suffix):
                 dict(m=None), dict(ldm=3), dict(index=None)):
         assert call(**bad) == INVALID, bad
     assert call(v=2 ** 31, ldx=2 ** 31, ldy=2 ** 31, ldm=2 ** 26) == UNSUPPORTED
+    assert call(w=2 ** 24, ldx=2 ** 31, ldy=2 ** 31) == UNSUPPORTED
     assert call(most=131072, ldt=131072, k=8192, ldbt=8192, ldbv=8192) == UNSUPPORTED
 
 
