@@ -148,16 +148,16 @@ inline int compute_units()
 }
 
 // Workgroups of `threads` threads running `kernel` that the current device holds at
-// once.  Queried once per (kernel, device); the cache is the only process-wide
+// once.  Queried once per (kernel, threads, device); the cache is the only process-wide
 // state of the library besides the call-tag counter and holds hardware facts only.
 template <typename K>
 inline int resident_blocks(K kernel, int threads)
 {
   static std::mutex mu;
-  static std::map<std::pair<const void*, int>, int> cache;
+  static std::map<std::pair<const void*, std::pair<int, int>>, int> cache;
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) return 0;
-  const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), dev);
+  const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), std::make_pair(threads, dev));
   std::lock_guard<std::mutex> lock(mu);
   auto it = cache.find(key);
   if (it != cache.end()) return it->second;
