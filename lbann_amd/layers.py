@@ -918,9 +918,9 @@ class residual_norm_layer(_Dropout):
         u = N1(branch);  v = dropout(u);  h = a * residual + b * gate * v;  y = N2(h)
 
     with N1 (`branch_norm`) and N2 (`output_norm`) "none", "rms" or "layer".  scale / bias arguments
-    are arrays or device tensors of `size` fp32 values, None for no such weight; scales default
-    to one where a norm is chosen and `None` is given.  branch, residual, h and y share one
-    storage type: fp32, fp16 or bfloat16.
+    are arrays or tensors of `size` values, None for no such weight (a scale of one, a bias of zero, and no
+    gradient); contiguous fp32 tensors on the device are used where they are, so that an optimizer's updates
+    are seen, others are copied.  branch, residual, h and y share one storage type: fp32, fp16 or bfloat16.
 
     forward(branch, residual, gate) returns y (None without an output norm) and keeps the new
     stream in `residual`; backward(dy, dresidual) returns (dbranch, dresidual of the old stream)

@@ -254,6 +254,67 @@ def test_residual_norm_not_finite(L):
     assert np.array_equal(np.isnan(h), kept) and (h[~kept] == 0).all()
 
 
+@pytest.mark.parametrize("n", [100, 1000, 1001, 2050, 6001, 9000, 20001])
+def test_residual_norm_not_finite_in_partly_filled_teams(L, n):
+    """Lanes without entries add nothing, also where the column holds an infinity: RMS norms give 0 for its finite
+    entries, forward and in the columns beside it backward."""
+    t = 5
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    o, dy = (torch.randn(t, n, generator=gen, device="cuda") for _ in range(2))
+    o[1, n - 1] = float("inf")
+    o[3, 0] = float("-inf")
+    A = L.DeviceMatrix.attach
+    layer = L.residual_norm_layer(n, "rms", "rms", branch_scale=np.ones(n), output_scale=np.ones(n))
+    y = layer.forward(A(o, n)).tensor
+    rows = torch.tensor([0, 2, 4], device="cuda")
+    assert torch.isfinite(y[rows]).all() and torch.isnan(y[1, n - 1]) and torch.isnan(y[3, 0])
+    h = layer.residual.tensor
+    assert (h[1, :n - 1] == 0).all() and (h[3, 1:] == 0).all()
+    db, _ = layer.backward(A(dy, n))
+    clean = L.residual_norm_layer(n, "rms", "rms", branch_scale=np.ones(n), output_scale=np.ones(n))
+    yc = clean.forward(A(o[rows].clone(), n)).tensor
+    dc, _ = clean.backward(A(dy[rows].clone(), n))
+    assert torch.equal(yc, y[rows]) and torch.equal(dc.tensor, db.tensor[rows])
+
+
+@pytest.mark.parametrize("n,t,gates", [(72, 1200, 3), (1001, 600, 40), (4096, 520, 5), (12288, 40, 8)])
+def test_residual_norm_gradients_not_wanted(L, n, t, gates):
+    """Calls of the C ABI that leave gradients out give the same for the others."""
+    rng = np.random.default_rng(n)
+    p, layer, gate, _, data = make(L, rng, n, t, ("layer", "rms", gates, 0.9, True), "bf16", 0, 0)
+    layer.forward(data["o"][0], data["r"][0], gate, offset=5)
+    db, dr = layer.backward(data["dy"][0], data["dh"][0])
+    want = {"db": db.tensor, "dr": dr.tensor, "dg": layer.m_gate_gradient.tensor,
+            **{i: getattr(layer, f"m_{k}_gradient").tensor for i, k in enumerate(("branch_scale", "branch_bias", "output_scale", "output_bias"))}}
+    lib, b, w = L.capi.lib(), L._buffer, layer.weights
+    for wanted in (set(), {"dg"}, {2}, {0, 3}, {"dr", 1}, {"dr", "dg", 0, 1, 2, 3}):
+        got_ = {k: torch.full_like(v, float("nan")) for k, v in want.items()}
+        m = {k: L.DeviceMatrix.attach(got_[k], n) if k in wanted or k == "db" else None for k in ("db", "dr", "dg")}
+        grads = [got_[i].data_ptr() if i in wanted else None for i in range(4)]
+        need = lib.lbn_residual_norm_bwd_workspace_bytes(n, t, int(any(grads)), gates if "dg" in wanted else 0, 2)
+        ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")   # NaN everywhere: nothing is read unwritten
+        L.call("lbn_residual_norm_bwd_bf16", L._stream(), n, t, 2, 1, p["epsilon"], p["a"], p["b"], *b(data["o"][0]), *b(layer.h),
+               *b(gate), gate.width, w["branch_scale"].data_ptr(), w["branch_bias"].data_ptr(), w["output_scale"].data_ptr(), 0.9, 77, 5, None,
+               3, *b(layer.m_statistics), *b(data["dy"][0]), *b(data["dh"][0]), *b(m["db"]), *b(m["dr"]), *b(m["dg"]), *grads,
+               ws.data_ptr(), need)
+        for k, v in want.items():
+            if k in wanted or k == "db":
+                if got_[k].dtype == torch.bfloat16:
+                    assert torch.equal(got_[k], v), (wanted, k)
+                else:   # ranges depend on what is wanted, and sums with them: both are within the bound of the same value
+                    off = (got_[k].double() - v.double()).abs()
+                    assert (off <= 2 * ref.roundings(n, t) * ref.U * sums_size(layer, p, data, gate, k)).all(), (wanted, k)
+            else:
+                assert torch.isnan(got_[k].float()).all(), (wanted, k)
+
+
+def sums_size(layer, p, data, gate, which):
+    o, dy, dh = data["o"], data["dy"], data["dh"]
+    want = ref.backward(o[1], got(layer.h), got(gate), got(layer.m_statistics), dy[1], dh[1], p, True)
+    name = {"dg": "dgate", 0: "dbranch_scale", 1: "dbranch_bias", 2: "doutput_scale", 3: "doutput_bias"}[which]
+    return torch.from_numpy(want[name][1] + np.abs(want[name][0])).cuda()
+
+
 # ---------------------------------------------------------------- logits
 LOGITS = [  # vocabulary, sequences, history, biases, masks, pad, shift
     (1, 1, 1, 1, 1, 0, 0), (7, 3, 0, 0, 0, 0, 0), (33, 5, 50, 3, 2, 1, 1), (1000, 4, 300, 17, 4, 0, 0), (4095, 2, 5000, 0, 1, 3, 0),
