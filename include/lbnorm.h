@@ -812,7 +812,8 @@ int lbn_residual_norm_fwd_bf16(lbn_stream_t stream, int64_t size, int64_t width,
  * (NULL: not wanted), both may take the place of dy, dh, h or branch of the same leading
  * dimension.  dgate (size x num_gates), dbranch_scale, dbranch_bias, doutput_scale,
  * doutput_bias: overwritten where non-NULL (NULL: not wanted; must be NULL for a norm that is
- * LBN_NORM_NONE, dgate without a gate).
+ * LBN_NORM_NONE, dgate without a gate).  As any call, one with width 0 launches nothing and writes nothing: a
+ * caller whose share of a mini-batch may be empty clears these sums itself.
  * The workspace is lbn_residual_norm_bwd_workspace_bytes() large, 16-byte aligned:
  * has_weight_grads != 0 if any of the four weight gradients is wanted, num_gate_grads =
  * num_gates if dgate is, else 0, elem_bytes 4 or 2 for the storage type. */

@@ -1312,7 +1312,8 @@ public:
     for (int kind : {branch_norm, output_norm})
       if (kind < LBN_NORM_NONE || kind > LBN_NORM_LAYER) throw exception("residual_norm_layer: unknown norm kind");
   }
-  /// Weight vectors of the two norms (device memory, NULL for 1 resp. 0) and their gradients (NULL: not wanted).
+  /// Weight vectors of the two norms (device memory, NULL for 1 resp. 0) and their gradients (NULL: not wanted;
+  /// left as they are by a backward of width 0).
   void set_weights(const float* branch_scale, const float* branch_bias, const float* output_scale, const float* output_bias)
   {
     m_w[0] = branch_scale, m_w[1] = branch_bias, m_w[2] = output_scale, m_w[3] = output_bias;

@@ -995,7 +995,9 @@ class residual_norm_layer(_Dropout):
     def bind_saved(self, branch, h, statistics, gate=None, has_residual=True, offset=0, training=True):
         """What an earlier forward left behind, for a backward without one in this object
         (recomputation, pipelines): its block output, new stream, statistics, gate and dropout offset."""
-        self._check_gate(gate, h)
+        if statistics is None:
+            raise ValueError("bind_saved takes the statistics of a training-mode forward")
+        self._check_gate(gate, statistics)
         self.branch, self.h, self.m_statistics, self.gate = branch, h, statistics, gate
         self.residual, self.m_has_residual = h, bool(has_residual)
         self._start(training, offset)
@@ -1024,6 +1026,10 @@ class residual_norm_layer(_Dropout):
             grads.append(None if g is None else g.tensor.data_ptr())
         gates = 0 if gate is None else gate.width
         self.m_gate_gradient = dgate = None if gate is None else _matrix_beside(like, n, gates, torch.float32)
+        if w == 0:  # nothing is launched then; sums over no columns are zero
+            for m in (dgate, *(getattr(self, attribute) for _, attribute in self._gradients)):
+                if m is not None:
+                    m.tensor.zero_()
         key = w, gates, like.tensor.dtype
         if self._scratch_for != key:
             self._scratch_for = key

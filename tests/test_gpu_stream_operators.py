@@ -542,6 +542,37 @@ def test_empty_calls(L):
     assert (y.tensor == 2).all()
 
 
+@pytest.mark.parametrize("n", [1, 3, 100, 1001, 20000])
+def test_gradients_of_an_empty_batch(L, n):
+    """The sums over no columns are zero, not what the memory held."""
+    layer = L.residual_norm_layer(n, "layer", "rms", branch_scale=np.ones(n), branch_bias=np.ones(n), output_scale=np.ones(n),
+                                  output_bias=np.ones(n))
+    none = L.DeviceMatrix(n, 0, dtype=torch.bfloat16)
+    layer.forward(none, none, L.DeviceMatrix(n, 3))
+    held = [torch.full((3 * n,), float("nan"), device="cuda") for _ in range(8)]   # what the gradients' memory may hold
+    del held
+    layer.backward(none, none)
+    names = ["m_branch_scale_gradient", "m_branch_bias_gradient", "m_output_scale_gradient", "m_output_bias_gradient", "m_gate_gradient"]
+    for name in names:
+        assert (getattr(layer, name).tensor == 0).all(), name
+
+
+def test_saved_state_without_the_new_stream(L):
+    """Without an output norm backward does not read the new stream, which need not be kept."""
+    n, t = 200, 12
+    rng = np.random.default_rng(8)
+    p, layer, gate, _, data = make(L, rng, n, t, ("layer", "none", 3, 0.8, True), "f16", 0, 0)
+    layer.forward(data["o"][0], data["r"][0], gate, offset=9)
+    db, dr = layer.backward(None, data["dh"][0])
+    dgate, statistics = layer.m_gate_gradient, layer.m_statistics
+    layer.bind_saved(data["o"][0], None, statistics, gate, offset=9)
+    db2, dr2 = layer.backward(None, data["dh"][0])
+    assert torch.equal(db.tensor, db2.tensor) and torch.equal(dr.tensor, dr2.tensor)
+    assert torch.equal(dgate.tensor, layer.m_gate_gradient.tensor)
+    with pytest.raises(ValueError):
+        layer.bind_saved(data["o"][0], None, None, gate)
+
+
 def test_residual_norm_in_place_while_training(L):
     """The new stream may take the old one's place in training too; the block's output is kept for backward."""
     n, t = 640, 9
