@@ -451,8 +451,8 @@ constexpr int kMergeRows = 3;
 // TB/s).  One workgroup a compute unit keeps the partial rows few (256 of them: 4.9 us to merge).
 //
 // TEAM: lanes of the largest team.  Up to 512 (256 registers a thread) the weights of a thread's unit stay in
-// registers beside its up to five sums; teams of up to 1024 (128 registers) with many sums read them
-// again for every column, from L2.
+// registers beside its up to five sums; teams of up to 1024 (128 registers) with many sums read the weights
+// again for every column, from L2, and keep all sums but one in LDS.
 template <typename T, int TEAM, bool BRANCH_NORM, bool GATE, bool BIAS, bool EVEN, bool STREAM>
 __global__ void __launch_bounds__(TEAM <= 512 ? 512 : 1024)
 rn_bwd_rows(RnBwdRows<T> a)
@@ -460,7 +460,10 @@ rn_bwd_rows(RnBwdRows<T> a)
   using U = Unit<T>;
   constexpr bool SUB = TEAM == 16;
   constexpr bool kKeepWeights = TEAM <= 512 || (!GATE && (sizeof(T) == 2 ? !(BRANCH_NORM && BIAS) : !BRANCH_NORM));
+  constexpr bool kLdsSums = !kKeepWeights;
   extern __shared__ __align__(16) float merged[];  // kMergeRows x blockDim x 8 floats if there are several teams
+  // 16-byte pieces of the sums that are not in registers: piece i of thread t at [i][t]
+  __shared__ v4f lds_sums[kLdsSums ? 2 * (kGrads - 1) : 1][kLdsSums ? TEAM : 1];
   __shared__ float* merged_rows[kMergeRows];
   __shared__ float2 slots[2][kMergeSlots];
   TeamMerge merge;
@@ -478,7 +481,11 @@ rn_bwd_rows(RnBwdRows<T> a)
   unsigned first, last;
   rn_range(blockIdx.x, width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
 
-  auto weights = [&](const float* w, float fill, float (&out)[8]) { share.weights(w, 0, fill, out); };
+  auto weights = [&](const float* w, float fill, float (&out)[8]) {
+    RowShare<1, EVEN> here = share;
+    if constexpr (!kKeepWeights) asm volatile("" : "+v"(here.at[0]));  // read now: not kept from the last column
+    here.weights(w, 0, fill, out);
+  };
   float w2[8], w1[8], b1[8], gt[8];
   const float* gate_row = a.gate;
   auto load_output_weights = [&] { weights(a.output_scale, 1.f, w2); };
@@ -496,6 +503,30 @@ rn_bwd_rows(RnBwdRows<T> a)
   }
 
   float acc[kGrads][8] = {};
+  // A thread's sum of quantity q: `next(j, sum)` is what entry j becomes.
+  auto update = [&](auto quantity, auto next) {
+    constexpr int q = decltype(quantity)::value;
+    if constexpr (kLdsSums && q > 0) {
+      v4f* const s = &lds_sums[2 * (q - 1)][threadIdx.x];
+      v4f low = s[0], high = s[TEAM];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) low[j] = next(j, low[j]), high[j] = next(4 + j, high[j]);
+      s[0] = low, s[TEAM] = high;
+    }
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[q][j] = next(j, acc[q][j]);
+    }
+  };
+  if constexpr (kLdsSums) {
+#pragma unroll
+    for (int i = 0; i < 2 * (kGrads - 1); ++i) lds_sums[i][threadIdx.x] = v4f{0.f, 0.f, 0.f, 0.f};
+  }
+  constexpr std::integral_constant<int, kGradOutputScale> output_scale_sum;
+  constexpr std::integral_constant<int, kGradOutputBias> output_bias_sum;
+  constexpr std::integral_constant<int, kGradBranchScale> branch_scale_sum;
+  constexpr std::integral_constant<int, kGradBranchBias> branch_bias_sum;
+  constexpr std::integral_constant<int, kGradGate> gate_sum;
   typename U::raw_t qy{}, qh{}, qs{}, qo{};
   RnColumnStats qstats{0.f, 1.f, 0.f, 1.f};
   auto issue = [&](unsigned col) {
@@ -517,8 +548,17 @@ rn_bwd_rows(RnBwdRows<T> a)
     constexpr int kFirst = decltype(first_q)::value, kLast = decltype(last_q)::value;
     if (teams == 1) {
 #pragma unroll
-      for (int q = kFirst; q <= kLast; ++q)
-        if (rows[q]) store_unit<EVEN>(rows[q] + entry, valid, acc[q]);
+      for (int q = kFirst; q <= kLast; ++q) {
+        if (!rows[q]) continue;
+        if constexpr (kLdsSums) {
+          if (q > 0) {
+            const v4f low = lds_sums[2 * (q - 1)][threadIdx.x], high = lds_sums[2 * (q - 1) + 1][threadIdx.x];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[q][j] = low[j], acc[q][4 + j] = high[j];
+          }
+        }
+        store_unit<EVEN>(rows[q] + entry, valid, acc[q]);
+      }
     }
     else {
       const int stride = 8 * lanes, quads = (n + 3) / 4;
@@ -594,8 +634,11 @@ rn_bwd_rows(RnBwdRows<T> a)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             x[j] = (x[j] - s.mean2) * s.rstd2;
-            acc[kGradOutputScale][j] = __builtin_fmaf(f[j], x[j], acc[kGradOutputScale][j]);
-            if (BIAS) acc[kGradOutputBias][j] += f[j];
+          }
+          update(output_scale_sum, [&](int j, float sum) { return __builtin_fmaf(f[j], x[j], sum); });
+          if (BIAS) update(output_bias_sum, [&](int j, float sum) { return sum + f[j]; });
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
             f[j] *= w2[j];
             sp += f[j];
             spx = __builtin_fmaf(f[j], x[j], spx);
@@ -615,10 +658,7 @@ rn_bwd_rows(RnBwdRows<T> a)
         store_unit<EVEN>(column(a.dresidual, col, a.ld_dresidual) + entry, valid, f);
       }
       // e becomes du; o the normalised branch
-      if constexpr (!kKeepWeights) {
-        load_branch_weights();
-        load_gate();
-      }
+      if constexpr (!kKeepWeights) load_branch_weights();
       const float scale = dropping ? a.branch_mult * a.drop.inverse_keep : a.branch_mult;
       float ev[8];  // the gate's gradient
 #pragma unroll
@@ -628,8 +668,12 @@ rn_bwd_rows(RnBwdRows<T> a)
         if (GATE) {
           const float u = BRANCH_NORM ? (BIAS ? __builtin_fmaf(o[j], w1[j], b1[j]) : o[j] * w1[j]) : o[j];
           ev[j] = e[j] * u;
-          e[j] *= gt[j];
         }
+      }
+      if constexpr (GATE) {
+        if constexpr (!kKeepWeights) load_gate();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] *= gt[j];
       }
       if (dropping) {
         uint32_t w[4];
@@ -641,17 +685,14 @@ rn_bwd_rows(RnBwdRows<T> a)
           if (GATE) ev[j] = kept ? ev[j] : 0.f;
         }
       }
-      if (GATE && active && read_branch) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[kGradGate][j] += ev[j];
-      }
+      if (GATE && active && read_branch) update(gate_sum, [&](int j, float sum) { return sum + ev[j]; });
       if (BRANCH_NORM) {
         float sp = 0.f, spu = 0.f;
         if (active) {
+          update(branch_scale_sum, [&](int j, float sum) { return __builtin_fmaf(e[j], o[j], sum); });
+          if (BIAS) update(branch_bias_sum, [&](int j, float sum) { return sum + e[j]; });
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            acc[kGradBranchScale][j] = __builtin_fmaf(e[j], o[j], acc[kGradBranchScale][j]);
-            if (BIAS) acc[kGradBranchBias][j] += e[j];
             e[j] *= w1[j];
             sp += e[j];
             spu = __builtin_fmaf(e[j], o[j], spu);
@@ -671,8 +712,7 @@ rn_bwd_rows(RnBwdRows<T> a)
       float* rows[kGrads] = {};
       rows[kGradGate] = column(a.dgate, gate, a.ld_dgate);
       flush(std::integral_constant<int, kGradGate>{}, std::integral_constant<int, kGradGate>{}, rows);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[kGradGate][j] = 0.f;
+      update(gate_sum, [](int, float) { return 0.f; });
     }
     begin = end;
   }
