@@ -35,6 +35,7 @@ struct RnMergeArgs {
   float* out[kGrads];
   int64_t n, ld_dgate;
   unsigned ranges, num_gates, ranges_per_gate;
+  bool few;  // partial rows a gate, see kMergeFew
 };
 
 // A workgroup sums 64 neighbouring features: kMergeGroups groups of kMergeLanes lanes (four features each)
@@ -42,6 +43,9 @@ struct RnMergeArgs {
 // Bound by latency: many groups, so that a thread has few loads and they are all in flight (256
 // rows of 4096 features, three vectors: 4.9 us; 11.0 us with 16 groups of 64 single features).
 constexpr int kMergeLanes = 16, kMergeGroups = 64;
+// Gates of few partial rows have a group each, without a tree (27 gates of 8 rows of 5760 features and two scales:
+// a workgroup each, 15.2 us; so, 5.7).
+constexpr unsigned kMergeFew = 16;
 
 static __global__ void __launch_bounds__(kMergeLanes * kMergeGroups)
 rn_merge(RnMergeArgs a)
@@ -49,9 +53,35 @@ rn_merge(RnMergeArgs a)
   __shared__ float sums[kMergeGroups][4 * kMergeLanes + 4];
   const int lane = threadIdx.x % kMergeLanes, group = threadIdx.x / kMergeLanes;
   const int64_t first_k = static_cast<int64_t>(blockIdx.x) * 4 * kMergeLanes, k = first_k + 4 * lane;
-  for (uint64_t item = blockIdx.y; item < uint64_t(kGradGate) + a.num_gates; item += gridDim.y) {
+  const unsigned gate_items = a.few ? (a.num_gates + kMergeGroups - 1) / kMergeGroups : a.num_gates;
+  for (uint64_t item = blockIdx.y; item < uint64_t(kGradGate) + gate_items; item += gridDim.y) {
     const int q = item < kGradGate ? static_cast<int>(item) : kGradGate;
     if (!a.out[q]) continue;
+    if (q == kGradGate && a.few) {
+      const uint64_t gate = (item - kGradGate) * kMergeGroups + group;
+      if (gate < a.num_gates && k < a.n) {
+        const float* from = a.part[q] + gate * a.ranges_per_gate * a.n + k;
+        float s[4] = {};
+        float* out = a.out[q] + gate * a.ld_dgate + k;
+        if (k + 4 <= a.n) {
+#pragma unroll 4
+          for (unsigned b = 0; b < a.ranges_per_gate; ++b) {
+            const typename Pack<float>::vec_t r = Pack<float>::load(from + b * a.n);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += r[j];
+          }
+          __builtin_memcpy(out, s, sizeof(s));
+        }
+        else {
+          for (int j = 0; k + j < a.n; ++j) {
+            float t = 0.f;
+            for (unsigned b = 0; b < a.ranges_per_gate; ++b) t += from[b * a.n + j];
+            out[j] = t;
+          }
+        }
+      }
+      continue;
+    }
     const unsigned gate = static_cast<unsigned>(item) - kGradGate;  // the partial rows from `first` to `last`
     uint64_t first = 0, last = a.ranges - 1;
     float* out = a.out[q];
@@ -203,7 +233,8 @@ static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t
   return p;
 }
 
-// The row kernel of a call.  Lengths that are no multiple of eight take the one that accumulates everything.
+// The row kernel of a call.  Lengths that are no multiple of eight with a gate take the one that accumulates
+// everything (without a gate that costs: 502 x 12100 bf16, two norms, 24.5 us against 19.3).
 template <typename T, int TEAM>
 static auto rn_bwd_kernel(bool norm, bool gate, bool bias, bool even, bool stream) -> void (*)(RnBwdRows<T>)
 {
@@ -212,7 +243,9 @@ static auto rn_bwd_kernel(bool norm, bool gate, bool bias, bool even, bool strea
     if (gate) return bias ? rn_bwd_rows<T, TEAM, N, true, true, true, S> : rn_bwd_rows<T, TEAM, N, true, false, true, S>;
     return bias ? rn_bwd_rows<T, TEAM, N, false, true, true, S> : rn_bwd_rows<T, TEAM, N, false, false, true, S>;
   };
-  if (!even) return norm ? rn_bwd_rows<T, TEAM, true, true, true, false, false> : rn_bwd_rows<T, TEAM, false, true, true, false, false>;
+  if (!even && gate) return norm ? rn_bwd_rows<T, TEAM, true, true, true, false, false> : rn_bwd_rows<T, TEAM, false, true, true, false, false>;
+  if (!even && norm) return bias ? rn_bwd_rows<T, TEAM, true, false, true, false, false> : rn_bwd_rows<T, TEAM, true, false, false, false, false>;
+  if (!even) return bias ? rn_bwd_rows<T, TEAM, false, false, true, false, false> : rn_bwd_rows<T, TEAM, false, false, false, false, false>;
   if (stream) return norm ? of(std::true_type{}, std::true_type{}) : of(std::false_type{}, std::true_type{});
   return norm ? of(std::true_type{}, std::false_type{}) : of(std::false_type{}, std::false_type{});
 }
@@ -372,7 +405,8 @@ static int rn_bwd(lbn_stream_t stream, RnBwdArgs<T> a, int64_t num_gates, double
   merge.n = a.n, merge.ld_dgate = ld_dgate, merge.ranges = static_cast<unsigned>(plan.ranges);
   merge.num_gates = merge.out[kGradGate] ? static_cast<unsigned>(num_gates) : 0;
   merge.ranges_per_gate = static_cast<unsigned>(plan.ranges_per_gate);
-  const int64_t items = kGradGate + int64_t(merge.num_gates);
+  merge.few = merge.num_gates > 1 && merge.ranges_per_gate <= kMergeFew;
+  const int64_t items = kGradGate + (merge.few ? ceil_div(merge.num_gates, kMergeGroups) : int64_t(merge.num_gates));
   const dim3 merge_grid(static_cast<unsigned>(ceil_div(a.n, 4 * kMergeLanes)), static_cast<unsigned>(items < 32768 ? items : 32768));
 
   hipStream_t st = as_stream(stream);

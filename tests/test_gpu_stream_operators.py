@@ -148,6 +148,23 @@ def test_residual_norm(L, n, t, pad, shift, kinds, dtype):
     check_backward(layer, p, gate_v, data, dtype, n, t)
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("n,t,kinds", [(4104, 620, ("layer", "rms", 4, 0.9, True)), (5761, 540, ("rms", "layer", 27, 0.5, False)),
+                                       (8192, 520, ("none", "rms", 20, 1.0, True)), (8189, 300, ("layer", "rms", 0, 0.9, True)),
+                                       (4097, 600, ("rms", "rms", 600, 1.0, False)), (502, 1200, ("rms", "layer", 0, 1.0, False)),
+                                       (1001, 2400, ("layer", "none", 0, 0.75, True)), (131, 3000, ("none", "layer", 100, 1.0, True))])
+def test_residual_norm_over_many_ranges(L, n, t, kinds, dtype):
+    """Several columns in each range, several ranges to a gate or several gates to a range, the widest teams."""
+    rng = np.random.default_rng(n + t)
+    p, layer, gate, gate_v, data = make(L, rng, n, t, kinds, dtype, 0, 0)
+    h, y, _, size_h, size_y = ref.forward(data["o"][1], data["r"][1], gate_v, p)
+    out = layer.forward(data["o"][0], data["r"][0], gate, offset=5)
+    close("h", got(layer.residual), h, size_h, dtype, ref.roundings(n))
+    if y is not None:
+        close("y", got(out), y, size_y, dtype, ref.roundings(n))
+    check_backward(layer, p, gate_v, data, dtype, n, t)
+
+
 @pytest.mark.parametrize("n,t", [(96, 9), (4096, 5), (40001, 1)])
 def test_residual_norm_optional_parts(L, n, t):
     """No residual stream, no gradient of the stream, no weights; inference without statistics."""
