@@ -177,7 +177,8 @@ struct RnBwdPlan {
   size_t sums_bytes, weight_bytes, gate_bytes;
   size_t total() const { return sums_bytes + weight_bytes + gate_bytes; }
   int threads() const { return (shape.sub ? 16 : kWave * shape.nw) * teams; }
-  // About `most` ranges that do not cut across the end of a gate's columns.
+  // Up to `most` ranges that do not cut across the end of a gate's columns.  A few more would be a second round of
+  // workgroups (1024 x 4400 bf16 with 22 gates: 264 ranges 23.0 us, 242 of them 15.7).
   void cut(int64_t width, int64_t gates, int64_t most)
   {
     cols_per_range = ceil_div(width, most);
@@ -187,6 +188,7 @@ struct RnBwdPlan {
       const int64_t per_gate = width / gates;
       if (per_gate > cols_per_range) {
         ranges_per_gate = ceil_div(per_gate, cols_per_range);
+        if (ranges_per_gate > most / gates) ranges_per_gate = most / gates;
         cols_per_range = ceil_div(per_gate, ranges_per_gate);
         ranges = gates * ranges_per_gate;
         return;

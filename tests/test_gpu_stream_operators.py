@@ -152,7 +152,8 @@ def test_residual_norm(L, n, t, pad, shift, kinds, dtype):
 @pytest.mark.parametrize("n,t,kinds", [(4104, 620, ("layer", "rms", 4, 0.9, True)), (5761, 540, ("rms", "layer", 27, 0.5, False)),
                                        (8192, 520, ("none", "rms", 20, 1.0, True)), (8189, 300, ("layer", "rms", 0, 0.9, True)),
                                        (4097, 600, ("rms", "rms", 600, 1.0, False)), (502, 1200, ("rms", "layer", 0, 1.0, False)),
-                                       (1001, 2400, ("layer", "none", 0, 0.75, True)), (131, 3000, ("none", "layer", 100, 1.0, True))])
+                                       (1001, 2400, ("layer", "none", 0, 0.75, True)), (131, 3000, ("none", "layer", 100, 1.0, True)),
+                                       (1024, 2200, ("none", "rms", 22, 1.0, False))])
 def test_residual_norm_over_many_ranges(L, n, t, kinds, dtype):
     """Several columns in each range, several ranges to a gate or several gates to a range, the widest teams."""
     rng = np.random.default_rng(n + t)
