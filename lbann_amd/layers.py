@@ -806,18 +806,23 @@ def _entry(name, dtype):
 def _same_kind(like, height, width, **matrices):
     """Every given matrix has the shape, the storage type and the device of `like`."""
     t = like.tensor
+    dtype, index = t.dtype, t.get_device()
     for name, m in matrices.items():
-        if m is not None and (m.height != height or m.width != width or m.tensor.dtype != t.dtype
-                              or m.tensor.get_device() != t.get_device()):
-            raise ValueError(f"{name} is {m.height} x {m.width} {m.dtype} on {m.tensor.device}; expected "
-                             f"{height} x {width} {t.dtype} on {t.device}")
+        if m is None:
+            continue
+        u = m.tensor
+        if m.height != height or m.width != width or u.dtype is not dtype or u.get_device() != index:
+            raise ValueError(f"{name} is {m.height} x {m.width} {m.dtype} on {u.device}; expected "
+                             f"{height} x {width} {dtype} on {t.device}")
 
 
 def _stream_for(m):
     """The current stream, as an address.  Kernels go to the current device: refuse matrices of
     another one."""
     index = m.tensor.get_device()  # negative for host memory
-    if index < 0 or index != torch.cuda.current_device():
+    if index < 0:
+        raise ValueError(f"matrix on {m.tensor.device}; expected device memory")
+    if index != torch.cuda.current_device():
         raise ValueError(f"matrix on {m.tensor.device}; the current device is cuda:{torch.cuda.current_device()}")
     return torch._C._cuda_getCurrentRawStream(index)
 
@@ -825,8 +830,9 @@ def _stream_for(m):
 def _matrix_beside(like, height, width, dtype=None):
     """An uninitialised matrix on the device of `like`, of its storage type unless another is given."""
     m = DeviceMatrix.__new__(DeviceMatrix)
-    m.height, m.width, m.ldim = height, width, max(height, 1)
-    m.tensor = like.tensor.new_empty((max(width, 1), m.ldim), dtype=dtype)
+    m.height, m.width, m.ldim = height, width, height or 1
+    shape = width or 1, height or 1
+    m.tensor = like.tensor.new_empty(shape) if dtype is None else like.tensor.new_empty(shape, dtype=dtype)
     return m
 
 
@@ -969,12 +975,20 @@ class residual_norm_layer(_Dropout):
             raise ValueError(f"gate is {gate.height} x {gate.width} {gate.dtype}; expected {self.size} rows of fp32 on "
                              f"{like.tensor.device} and a number of columns that divides {like.width}")
 
+    def _check_weights(self, like):
+        index, n, fp32 = like.tensor.get_device(), self.size, torch.float32
+        for name, t in self.weights.items():
+            if t is None or t.get_device() == index and t.numel() == n and t.dtype is fp32 and t.is_contiguous():
+                continue
+            raise ValueError(f"{name}: {t.numel()} {t.dtype} values on {t.device}; expected {n} contiguous ones of fp32 on {like.tensor.device}")
+
     def forward(self, branch, residual=None, gate=None, training=True, offset=None, in_place=False):
         """in_place: the new stream overwrites `residual`, and outside training, where no backward
         needs it, y overwrites `branch`.  training=False: no dropout, no statistics."""
         n, w, kinds, wt = self.size, branch.width, self._kinds, self.weights
         _same_kind(branch, n, w, branch=branch, residual=residual)
         stream = _stream_for(branch)
+        self._check_weights(branch)
         self._check_gate(gate, branch)
         self._start(training, offset)
         self.branch, self.gate, self.m_has_residual = branch, gate, residual is not None
@@ -1014,6 +1028,7 @@ class residual_norm_layer(_Dropout):
         if st.height != 4 or st.width != w or st.tensor.dtype != torch.float32 or st.tensor.get_device() != like.tensor.get_device():
             raise ValueError("the statistics are a (4 x width) fp32 matrix")
         stream = _stream_for(like)
+        self._check_weights(like)
         dbranch = _matrix_beside(like, n, w)
         dres = _matrix_beside(like, n, w) if self.m_has_residual else None
         wanted = sum(wt[name] is not None for name, _ in self._gradients)
@@ -1035,11 +1050,11 @@ class residual_norm_layer(_Dropout):
             for m in (dgate, *(getattr(self, attribute) for _, attribute in self._gradients)):
                 if m is not None:
                     m.tensor.zero_()
-        key = w, gates, like.tensor.dtype
+        key = w, gates, like.tensor.dtype, wanted > 0
         if self._scratch_for != key:
             self._scratch_for = key
             self._scratch_bytes = capi.lib().lbn_residual_norm_bwd_workspace_bytes(
-                n, w, int(any(t is not None for t in wt.values())), gates, like.tensor.element_size())
+                n, w, int(wanted > 0), gates, like.tensor.element_size())
         need = self._scratch_bytes
         # scratch of this call alone: nothing that another stream or a recorded graph could share
         ws = like.tensor.new_empty((need,), dtype=torch.uint8) if need else None

@@ -545,6 +545,29 @@ def test_layers_refuse_another_place(L):
         L.residual_norm_layer(8).forward(x, gate=L.DeviceMatrix(8, 3))
 
 
+def test_weights_of_another_place(L):
+    """Weights are looked at in every call: host memory and wrong sizes are refused, new ones are used."""
+    n = 24
+    x = L.DeviceMatrix(n, 5, fill=1.0)
+    with pytest.raises(ValueError, match="output_scale"):
+        L.residual_norm_layer(n, output_scale=np.ones(n), device="cpu").forward(x)
+    layer = L.residual_norm_layer(n)
+    layer.forward(x)
+    layer.backward(x)
+    for bad in (torch.ones(n - 1, device="cuda"), torch.ones(n, device="cuda", dtype=torch.bfloat16), torch.ones(2 * n, device="cuda")[::2],
+                torch.ones(n)):
+        layer.weights["output_scale"] = bad
+        with pytest.raises(ValueError):
+            layer.forward(x)
+        with pytest.raises(ValueError):
+            layer.backward(x)
+    layer.weights["output_scale"] = torch.full((n,), 2.0, device="cuda")
+    y = layer.forward(x).tensor
+    assert (y == 2 * L.residual_norm_layer(n).forward(x).tensor).all()
+    layer.backward(x)
+    assert layer.m_output_scale_gradient.tensor.shape == (n,) and torch.isfinite(layer.m_output_scale_gradient.tensor).all()
+
+
 def test_empty_calls(L):
     """No columns, or no sequences: nothing happens, nothing fails."""
     layer = L.residual_norm_layer(16, "rms", "rms", output_scale=np.ones(16))

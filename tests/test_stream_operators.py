@@ -193,3 +193,13 @@ def test_dropout_offsets_advance():
         d._start(training, offset)
         taken.append((d.m_offset, d.m_kept))
     assert taken == [(0, 0.5), (1, 0.5), (1, 1.0), (40, 0.5), (2, 0.5)]
+
+
+def test_layers_refuse_host_memory():
+    """Without a GPU too: a refusal, not an error of the runtime."""
+    from lbann_amd import layers as L
+    host = L.DeviceMatrix(8, 2, device="cpu")
+    weights = L.residual_norm_layer(8, output_scale=np.ones(8), device="cpu")
+    for call in (lambda: L.dropout_layer(0.5).forward(host), lambda: L.logits_adjust_layer(8).forward(host), lambda: weights.forward(host)):
+        with pytest.raises(ValueError, match="device memory"):
+            call()
