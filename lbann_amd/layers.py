@@ -117,6 +117,22 @@ class _Vector:
         return self.tensor[: self.n].cpu().numpy()
 
 
+_STORAGE = {torch.float32: "f32", torch.float16: "f16", torch.float64: "f64"}
+
+
+def _storage(owner, types, *matrices):
+    """Suffix of the entry points for the storage type that every matrix of a call has (None: no such matrix).  A type
+    that the layer has no kernels for, bfloat16 among them, is refused: read as another type it would reach past its end."""
+    kinds = {m.tensor.dtype for m in matrices if m is not None}
+    if len(kinds) != 1:
+        raise TypeError(f"{type(owner).__name__}: matrices of different types {sorted(map(str, kinds))}")
+    suffix = _STORAGE.get(kinds.pop())
+    if suffix not in types:
+        raise TypeError(f"{type(owner).__name__}: storage is {' or '.join(types)}, not "
+                        f"{next(m.tensor.dtype for m in matrices if m is not None)}")
+    return suffix
+
+
 def _stream():
     return capi.vp(torch.cuda.current_stream().cuda_stream)
 
@@ -269,10 +285,8 @@ class layer_norm_layer(_Layer):
         self.m_statistics_gradient = None
         self.stats_mode = stats_mode
 
-    def _suffix(self):
-        if self.datatype == torch.float64:
-            return "f64"
-        return "f16" if self.prev_activations.dtype == torch.float16 else "f32"
+    def _suffix(self, *matrices):
+        return _storage(self, ("f64",) if self.datatype == torch.float64 else ("f32", "f16"), *matrices)
 
     def _scratch(self):
         """One scratch buffer for both directions, sized for the larger need, so that neither
@@ -291,6 +305,7 @@ class layer_norm_layer(_Layer):
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        suffix = self._suffix(x, y)
         G, n = self.num_normalized, self.normalization_size
         if self.m_statistics is None or self.m_statistics.width != x.width:
             self.m_statistics = DeviceMatrix(2 * G, x.width, dtype=self.datatype, device=self.device)
@@ -302,13 +317,14 @@ class layer_norm_layer(_Layer):
                     (_stream(), G, n, self.normalization_stride, x.width,
                      self.m_epsilon, x.Buffer(), x.ldim, y.Buffer(), y.ldim, self.m_statistics.Buffer(),
                      self.m_statistics.ldim, scale, bias, self.stats_mode))
-        return (f"lbn_layer_norm_fwd_{self._suffix()}",
+        return (f"lbn_layer_norm_fwd_{suffix}",
                 (_stream(), G, n, self.normalization_stride, x.width,
                  self.m_epsilon, x.Buffer(), x.ldim, y.Buffer(), y.ldim, self.m_statistics.Buffer(),
                  self.m_statistics.ldim, scale, bias, ws, nb, self.stats_mode))
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        suffix = self._suffix(x, dy, dx)
         G, n = self.num_normalized, self.normalization_size
         if self.m_statistics_gradient is None or self.m_statistics_gradient.width != x.width:
             self.m_statistics_gradient = DeviceMatrix(2 * G, x.width, dtype=self.datatype, device=self.device)
@@ -316,7 +332,7 @@ class layer_norm_layer(_Layer):
         dscale = self.m_scale_gradient.Buffer() if self.m_scale else _null()
         dbias = self.m_bias_gradient.Buffer() if self.m_bias else _null()
         ws, nb = self._scratch()
-        return (f"lbn_layer_norm_bwd_{self._suffix()}",
+        return (f"lbn_layer_norm_bwd_{suffix}",
                 (_stream(), G, n, self.normalization_stride, x.width,
                  self.m_epsilon, x.Buffer(), x.ldim, dy.Buffer(), dy.ldim, dx.Buffer(), dx.ldim,
                  self.m_statistics.Buffer(), self.m_statistics.ldim, self.m_statistics_gradient.Buffer(),
@@ -338,6 +354,7 @@ class instance_norm_layer(_Layer):
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        _storage(self, ("f32",), x, y)
         if self.m_workspace is None or self.m_workspace.width != x.width:
             self.m_workspace = DeviceMatrix(2 * self.num_channels, x.width, device=self.device)
         ws, nb = self._ws_fwd.get(capi.lib().lbn_instance_norm_fwd_workspace_bytes(
@@ -348,6 +365,7 @@ class instance_norm_layer(_Layer):
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32",), x, dy, dx)
         ws, nb = self._ws.get(capi.lib().lbn_instance_norm_bwd_workspace_bytes(
             self.num_channels, self.channel_size, x.width), self.device)
         return ("lbn_instance_norm_bwd_f32",
@@ -386,6 +404,7 @@ class entrywise_batch_normalization_layer(_Layer):
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        _storage(self, ("f32",), x, y)
         st = self.m_batch_statistics
         ws, nb = self._scratch()
         return ("lbn_entrywise_batch_norm_fwd_f32",
@@ -395,6 +414,7 @@ class entrywise_batch_normalization_layer(_Layer):
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32",), x, dy, dx)
         st, sg = self.m_batch_statistics, self.m_batch_statistics_gradient
         ws, nb = self._scratch()
         return ("lbn_entrywise_batch_norm_bwd_f32",
@@ -409,6 +429,7 @@ class entrywise_batch_normalization_layer(_Layer):
         if self.comm_allreduce is None:
             return super().fp_compute()
         x, y, st = self.prev_activations, self.activations, self.m_batch_statistics
+        _storage(self, ("f32",), x, y)
         if self.training:
             count = int(self.statistics_count if self.statistics_count is not None else x.width)
             call("lbn_entrywise_batch_norm_fwd_sums_f32", _stream(), x.height, x.width, x.Buffer(), x.ldim,
@@ -426,6 +447,7 @@ class entrywise_batch_normalization_layer(_Layer):
         if self.comm_allreduce is None or not self.training:
             return super().bp_compute()
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32",), x, dy, dx)
         st, sg = self.m_batch_statistics, self.m_batch_statistics_gradient
         count = int(self.statistics_count if self.statistics_count is not None else x.width)
         if count > 1:
@@ -474,16 +496,15 @@ class batch_normalization_layer(_Layer):
             return self._ws.get(capi.lib().lbn_batch_norm_workspace_bytes_f64(C, cs, width), self.device)
         return self._ws.get(capi.lib().lbn_batch_norm_workspace_bytes(C, cs, width), self.device)
 
-    def _suffix(self, x):
-        if self.datatype == torch.float64:
-            return "f64"
-        return "f16" if x.dtype == torch.float16 else "f32"
+    def _suffix(self, *matrices):
+        return _storage(self, ("f64",) if self.datatype == torch.float64 else ("f32", "f16"), *matrices)
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        suffix = self._suffix(x, y)
         C, cs = self.num_channels, self.channel_size
         ws, nb = self._scratch(x.width)
-        return (f"lbn_batch_norm_fwd_{self._suffix(x)}",
+        return (f"lbn_batch_norm_fwd_{suffix}",
                 (_stream(), C, cs, x.width, int(self.m_bessel_correction),
                  self.m_epsilon, self.m_decay, int(self.training), x.Buffer(), x.ldim, y.Buffer(), y.ldim,
                  self._col(self.m_mean_and_var, 0), self._col(self.m_mean_and_var, 1),
@@ -492,10 +513,12 @@ class batch_normalization_layer(_Layer):
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        suffix = self._suffix(x, dy, dx)
         C, cs = self.num_channels, self.channel_size
         ws, nb = self._scratch(x.width)
-        name = f"lbn_batch_norm_bwd_{self._suffix(x)}"
+        name = f"lbn_batch_norm_bwd_{suffix}"
         if self.stats_mode & LBN_STATS_REFERENCE_ORDER and self.datatype != torch.float64:  # parity tests: the reference's order of summation
+            _storage(self, ("f32",), x)
             name = "lbn_batch_norm_bwd_reference_order_f32"
         return (name,
                 (_stream(), C, cs, x.width, int(self.m_bessel_correction),
@@ -509,25 +532,26 @@ class batch_normalization_layer(_Layer):
 class _softmax_like(_Layer):
     _name = None
 
-    @staticmethod
-    def _suffix(m):
-        return {torch.float16: "f16", torch.float64: "f64"}.get(m.dtype, "f32")
+    def _suffix(self, *matrices):
+        return _storage(self, ("f32", "f16", "f64"), *matrices)
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        suffix = self._suffix(x, y)
         if x.dtype == torch.float64:  # TensorDataType = double: no scratch
             return (f"lbn_{self._name}_fwd_f64", (_stream(), x.height, x.width, x.Buffer(), x.ldim, y.Buffer(), y.ldim))
         ws, nb = self._ws.get(capi.lib().lbn_softmax_workspace_bytes(x.height, x.width), self.device)
-        return (f"lbn_{self._name}_fwd_{self._suffix(x)}",
+        return (f"lbn_{self._name}_fwd_{suffix}",
                 (_stream(), x.height, x.width, x.Buffer(), x.ldim, y.Buffer(), y.ldim, ws, nb))
 
     def bp_call(self):
         y, dy, dx = self.activations, self.prev_error_signals, self.error_signals
+        suffix = self._suffix(y, dy, dx)
         if y.dtype == torch.float64:
             return (f"lbn_{self._name}_bwd_f64",
                     (_stream(), y.height, y.width, y.Buffer(), y.ldim, dy.Buffer(), dy.ldim, dx.Buffer(), dx.ldim))
         ws, nb = self._ws.get(capi.lib().lbn_softmax_workspace_bytes(y.height, y.width), self.device)
-        return (f"lbn_{self._name}_bwd_{self._suffix(y)}",
+        return (f"lbn_{self._name}_bwd_{suffix}",
                 (_stream(), y.height, y.width, y.Buffer(), y.ldim, dy.Buffer(), dy.ldim, dx.Buffer(),
                  dx.ldim, ws, nb))
 
@@ -575,6 +599,7 @@ class channelwise_softmax_layer(_Layer):
 
     def fp_call(self):
         x, y = self.prev_activations, self.activations
+        _storage(self, ("f32", "f64"), x, y)
         cs, stride, C = self.get_channel_size_and_stride()
         if x.dtype == torch.float64:
             return ("lbn_channelwise_softmax_fwd_f64",
@@ -585,6 +610,7 @@ class channelwise_softmax_layer(_Layer):
 
     def bp_call(self):
         y, dy, dx = self.activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32", "f64"), y, dy, dx)
         cs, stride, C = self.get_channel_size_and_stride()
         if y.dtype == torch.float64:
             return ("lbn_channelwise_softmax_bwd_f64",
@@ -621,11 +647,13 @@ class entrywise_scale_bias_layer(_scale_bias_layer):
 
     def fp_call(self):
         x, y, wt = self.prev_activations, self.activations, self.weights
+        _storage(self, ("f32",), x, y)
         return ("lbn_entrywise_scale_bias_fwd_f32",
                 (_stream(), x.height, x.width, x.Buffer(), x.ldim, y.Buffer(), y.ldim, wt.Buffer(), wt.ldim))
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32",), x, dy, dx)
         wt, wg = self.weights, self.m_weights_gradient
         self._ws.header = False
         ws, nb = self._ws.get(capi.lib().lbn_entrywise_scale_bias_bwd_workspace_bytes(x.height, x.width),
@@ -647,12 +675,14 @@ class channelwise_scale_bias_layer(_scale_bias_layer):
 
     def fp_call(self):
         x, y, wt = self.prev_activations, self.activations, self.weights
+        _storage(self, ("f32",), x, y)
         return ("lbn_channelwise_scale_bias_fwd_f32",
                 (_stream(), self.num_channels, self.channel_size, x.width, x.Buffer(), x.ldim, y.Buffer(), y.ldim,
                  wt.Buffer(), wt.ldim))
 
     def bp_call(self):
         x, dy, dx = self.prev_activations, self.prev_error_signals, self.error_signals
+        _storage(self, ("f32",), x, dy, dx)
         wt, wg = self.weights, self.m_weights_gradient
         C, cs = self.num_channels, self.channel_size
         self._ws.header = False
@@ -682,19 +712,16 @@ class cross_entropy_layer:
         self.error_signals = [None, None]
         self._ws = _Workspace("cross_entropy_layer", header=False)
 
-    @staticmethod
-    def _suffix(*matrices):
+    def _suffix(self, *matrices):
         """fp32 or fp16 storage (the reference instantiates the layer for both,
         cross_entropy.cpp:157-166); every matrix of a call has the layer's one data type."""
-        kinds = {m.dtype for m in matrices if m is not None}
-        if len(kinds) != 1:
-            raise TypeError(f"cross entropy: matrices of different types {sorted(map(str, kinds))}")
-        return "f16" if kinds.pop() == torch.float16 else "f32"
+        return _storage(self, ("f32", "f16"), *matrices)
 
     def fp_call(self):
         x, t, y = self.prev_activations[0], self.prev_activations[1], self.activations
+        suffix = self._suffix(x, t, y)
         ws, nb = self._ws.get(capi.lib().lbn_cross_entropy_fwd_workspace_bytes(x.height, x.width), self.device)
-        return (f"lbn_cross_entropy_fwd_{self._suffix(x, t, y)}",
+        return (f"lbn_cross_entropy_fwd_{suffix}",
                 (_stream(), x.height, x.width, int(self.m_use_labels), self.spatial_sample_size, x.Buffer(), x.ldim,
                  t.Buffer(), t.ldim, y.Buffer(), y.ldim, ws, nb))
 
@@ -740,8 +767,7 @@ def softmax_cross_entropy_forward(softmax, cross_entropy, x, ground_truth):
     cross_entropy.forward(y, ground_truth) computes, with both layers' members bound as
     those two calls bind them, so each layer's backward runs unchanged afterwards.
     Returns (y, loss).  fp32 storage only."""
-    if x.dtype != torch.float32:
-        raise TypeError("softmax_cross_entropy_forward takes fp32 matrices")
+    _storage(softmax, ("f32",), x, ground_truth)
     softmax.bind_forward(x)
     y = softmax.activations
     cross_entropy.prev_activations = [y, ground_truth]
@@ -764,6 +790,7 @@ def softmax_cross_entropy_backward(softmax, cross_entropy, dloss, want_dtruth=Fa
     y, truth = cross_entropy.prev_activations
     if y is not softmax.activations:
         raise ValueError("the softmax layer's output is not the cross-entropy layer's prediction")
+    _storage(cross_entropy, ("f32",), y, truth, dloss)
     cross_entropy.prev_error_signals = dloss
     dtruth = None
     if want_dtruth and not cross_entropy.m_use_labels:
@@ -1149,6 +1176,8 @@ class gradient_buffer:
         """contrib: a DeviceMatrix of the buffer's shape, or a _Vector / torch tensor holding one column
         (then `ldim` is its leading dimension when the buffer has several columns)."""
         g = self.gradient
+        if (contrib.tensor if hasattr(contrib, "tensor") else contrib).dtype != torch.float32:
+            raise TypeError("gradient contributions are fp32")
         buf_scale, in_scale = self._scales(sync_needed)
         if isinstance(contrib, DeviceMatrix):
             if (contrib.height, contrib.width) != (g.height, g.width):
