@@ -199,6 +199,24 @@ struct layer_io {
   hipStream_t stream = nullptr;
 };
 
+/// Storage of bfloat16 entries for applications without a type of their own.
+struct bfloat16 {
+  uint16_t bits;
+};
+
+/// Which entry points serve an element type: float, or a 2-byte type holding IEEE binary16 unless
+/// this trait is specialised (as below) to say that it holds bfloat16.
+enum class storage { f32, f16, bf16 };
+template <typename T>
+struct storage_of {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 2, "fp32, fp16 or bfloat16 storage");
+  static constexpr storage value = sizeof(T) == 4 ? storage::f32 : storage::f16;
+};
+template <>
+struct storage_of<bfloat16> {
+  static constexpr storage value = storage::bf16;
+};
+
 namespace detail {
 inline int64_t product(const std::vector<int64_t>& d, size_t from, size_t to)
 {
@@ -211,6 +229,13 @@ template <typename T> struct is_half : std::false_type {};
 /// fp16-storage entry points.
 template <typename Mat>
 using element_t = std::remove_cv_t<std::remove_pointer_t<decltype(std::declval<Mat&>().Buffer())>>;
+/// Whether a 2-byte type holds bfloat16, which the classes that know fp16 only must not take for it.
+template <typename T>
+constexpr bool holds_bfloat16()
+{
+  if constexpr (sizeof(T) == 2) return storage_of<T>::value == storage::bf16;
+  else return false;
+}
 }  // namespace detail
 
 // ------------------------------------------------------------------ layer norm
@@ -219,6 +244,8 @@ using element_t = std::remove_cv_t<std::remove_pointer_t<decltype(std::declval<M
 /// (TensorDataType = double: statistics, weights and their gradients are doubles too).
 template <typename T, typename Mat = device_matrix<T>>
 class layer_norm_layer {
+  static_assert(!detail::holds_bfloat16<T>() && !detail::holds_bfloat16<detail::element_t<Mat>>(),
+                "this layer has no bfloat16 kernels");
 public:
   /// Type of statistics, weights and weight gradients: float unless the layer is one of doubles.
   using weight_t = std::conditional_t<sizeof(T) == 8, double, float>;
@@ -369,6 +396,8 @@ private:
 template <typename T = float, typename Mat = device_matrix<T>>
 class batch_normalization_layer {
   static_assert(sizeof(T) == 8 || sizeof(T) == 4 || sizeof(T) == 2, "fp64, fp32 or fp16 storage");
+  static_assert(!detail::holds_bfloat16<T>() && !detail::holds_bfloat16<detail::element_t<Mat>>(),
+                "this layer has no bfloat16 kernels");
 public:
   using weight_t = std::conditional_t<sizeof(T) == 8, double, float>;
   batch_normalization_layer(double decay = 0.9, double epsilon = 1e-5, int statistics_group_size = 1,
@@ -510,6 +539,7 @@ enum class softmax_mode { INVALID, INSTANCE, CHANNEL };
 /// include/lbann/layers/activations/softmax.hpp:85-262, data-parallel layout.
 template <typename Mat = device_matrix<float>>
 class softmax_layer {
+  static_assert(!detail::holds_bfloat16<detail::element_t<Mat>>(), "this layer has no bfloat16 kernels");
 public:
   explicit softmax_layer(softmax_mode mode = softmax_mode::INSTANCE) : m_mode(mode)
   {
@@ -584,6 +614,7 @@ private:
 /// include/lbann/layers/activations/log_softmax.hpp.
 template <typename Mat = device_matrix<float>>
 class log_softmax_layer {
+  static_assert(!detail::holds_bfloat16<detail::element_t<Mat>>(), "this layer has no bfloat16 kernels");
 public:
   layer_io<Mat> io;
   void fp_compute()
@@ -925,6 +956,7 @@ private:
 /// (w.r.t. the prediction) and, without use_labels, ground_truth_error_signals.
 template <typename Mat = device_matrix<float>>
 class cross_entropy_layer {
+  static_assert(!detail::holds_bfloat16<detail::element_t<Mat>>(), "this layer has no bfloat16 kernels");
 public:
   explicit cross_entropy_layer(bool use_labels = false) : m_use_labels(use_labels) {}
 
@@ -1203,24 +1235,6 @@ private:
 
 
 // ------------------------------------------------- the residual stream and the logits
-/// Storage of bfloat16 entries for applications without a type of their own.
-struct bfloat16 {
-  uint16_t bits;
-};
-
-/// Which entry points serve an element type: float, or a 2-byte type holding IEEE binary16 unless
-/// this trait is specialised (as below) to say that it holds bfloat16.
-enum class storage { f32, f16, bf16 };
-template <typename T>
-struct storage_of {
-  static_assert(sizeof(T) == 4 || sizeof(T) == 2, "fp32, fp16 or bfloat16 storage");
-  static constexpr storage value = sizeof(T) == 4 ? storage::f32 : storage::f16;
-};
-template <>
-struct storage_of<bfloat16> {
-  static constexpr storage value = storage::bf16;
-};
-
 /// Where the random bits of a layer come from (include/lbnorm.h, lbn_dropout_*).  Every
 /// training-mode forward takes the next offset; backward repeats the last one.
 struct dropout_state {
@@ -1266,6 +1280,7 @@ void require_shape(const Mat* m, int64_t h, int64_t w, const char* what)
 /// from a counter in both directions and never stored.
 template <typename T = float, typename Mat = device_matrix<T>>
 class dropout_layer {
+  static_assert(sizeof(T) == sizeof(detail::element_t<Mat>), "T is the storage type of Mat's entries");
 public:
   explicit dropout_layer(double keep_prob = 0.5, uint64_t seed = 0)
   {
@@ -1303,6 +1318,7 @@ private:
 /// h = a residual + b gate v, y = N2(h) (include/lbnorm.h, lbn_residual_norm_*).
 template <typename T = float, typename Mat = device_matrix<T>, typename Mat32 = device_matrix<float>>
 class residual_norm_layer {
+  static_assert(sizeof(T) == sizeof(detail::element_t<Mat>), "T is the storage type of Mat's entries");
 public:
   residual_norm_layer(int branch_norm = LBN_NORM_NONE, int output_norm = LBN_NORM_RMS, double epsilon = 1e-5,
                       double residual_multiplier = 1.0, double branch_multiplier = 1.0)
@@ -1411,6 +1427,7 @@ private:
 template <typename T = float, typename Mat = device_matrix<T>, typename MatInt = device_matrix<int32_t>,
           typename Mat32 = device_matrix<float>>
 class logits_adjust_layer {
+  static_assert(sizeof(T) == sizeof(detail::element_t<Mat>), "T is the storage type of Mat's entries");
 public:
   hipStream_t stream = nullptr;
   const Mat* logits = nullptr;      // vocabulary x sequences
