@@ -1352,11 +1352,12 @@ public:
   Mat32* gate_gradient = nullptr;       // may stay null
   dropout_state state;
   bool is_training = true;
-  device_matrix<float> m_statistics;    // 4 x width, written in training mode
+  device_matrix<float> m_statistics;    // 4 x width, written in training mode; no columns after any other forward
 
   void fp_compute()
   {
     const char* where = "residual_norm_layer::fp_compute";
+    m_statistics.Resize(4, 0);  // those of an earlier call do not describe what is bound now; their memory stays
     if (!branch) throw exception("residual_norm_layer::fp_compute: no branch");
     const int64_t n = branch->Height(), w = branch->Width();
     detail::require_shape(residual, n, w, "residual");
@@ -1367,12 +1368,14 @@ public:
     if (is_training) m_statistics.Resize(4, w);
     const auto entry = detail::pick<storage_of<T>::value>(lbn_residual_norm_fwd_f32, lbn_residual_norm_fwd_f16,
                                                           lbn_residual_norm_fwd_bf16);
-    check_status(entry(stream, n, w, m_branch_norm, m_output_norm, m_epsilon, m_a, m_b, detail::in<T>(branch),
-                       branch->LDim(), detail::in<T>(residual), detail::ld(residual), gate_buffer(), detail::ld(gate),
-                       gates(), m_w[0], m_w[1], m_w[2], m_w[3], state.kept, state.seed, state.offset, state.step,
-                       state.column_offset, detail::out<T>(new_residual), detail::ld(new_residual), detail::out<T>(output),
-                       detail::ld(output), is_training ? m_statistics.Buffer() : nullptr, m_statistics.LDim()),
-                 where);
+    const int status =
+      entry(stream, n, w, m_branch_norm, m_output_norm, m_epsilon, m_a, m_b, detail::in<T>(branch), branch->LDim(),
+            detail::in<T>(residual), detail::ld(residual), gate_buffer(), detail::ld(gate), gates(), m_w[0], m_w[1], m_w[2],
+            m_w[3], state.kept, state.seed, state.offset, state.step, state.column_offset, detail::out<T>(new_residual),
+            detail::ld(new_residual), detail::out<T>(output), detail::ld(output),
+            is_training ? m_statistics.Buffer() : nullptr, m_statistics.LDim());
+    if (status != LBN_OK) m_statistics.Resize(4, 0);
+    check_status(status, where);
   }
 
   void bp_compute()

@@ -596,6 +596,44 @@ int drv_stream_error_cases(void)
   return missed;
 }
 
+// A backward after a forward that left no statistics, where an earlier one had: matrices without rows, so
+// that every call that is made succeeds without a device.
+int drv_stale_statistics(void)
+{
+  int missed = 0;
+  device_matrix<float> a, wide;
+  a.Attach(0, 6, nullptr, 1), wide.Attach(0, 5, nullptr, 1);
+  float four[24];
+  auto after_training = [&](residual_norm_layer<>& l) {
+    l.branch = &a, l.output = &a, l.new_residual = &a, l.output_gradient = &a, l.branch_gradient = &a;
+    l.m_statistics.Attach(4, 6, four, 4);
+  };
+  auto backward_refused = [&](residual_norm_layer<>& l) {
+    try { l.bp_compute(); }
+    catch (const exception& e) { return std::string(e.what()).find("training-mode forward") != std::string::npos; }
+    return false;
+  };
+  {
+    residual_norm_layer<> l;
+    after_training(l);
+    if (backward_refused(l)) ++missed;   // what was left there is used
+    l.is_training = false;
+    l.fp_compute();
+    if (!backward_refused(l)) ++missed;  // evaluation leaves none
+    after_training(l);
+    if (backward_refused(l)) ++missed;
+  }
+  {
+    residual_norm_layer<> l;
+    after_training(l);
+    l.residual = &wide;                  // a forward that is refused leaves none either
+    try { l.fp_compute(); ++missed; } catch (const exception&) {}
+    l.residual = nullptr;
+    if (!backward_refused(l)) ++missed;
+  }
+  return missed;
+}
+
 int drv_error_cases(void)
 {
   int missed = 0;
