@@ -769,7 +769,8 @@ int lbn_dropout_bwd_bf16(lbn_stream_t stream, int64_t height, int64_t width, dou
  *   stats: (4 x width) fp32: mean and variance of o, mean and variance of h (RMS: 0 and the mean of
  *   squares; no norm: 0 and 1), kept for backward; NULL if not wanted (inference).
  * Outputs may take the place of inputs of the same shape and leading dimension (h that of r or
- * o, y likewise).  Storage fp32, IEEE binary16 or bfloat16; arithmetic, statistics, weights,
+ * o, y likewise; h and y are two matrices).  With an output norm backward reads h, so in training the stream that one
+ * call returned must not be overwritten by the next before that backward has run.  Storage fp32, IEEE binary16 or bfloat16; arithmetic, statistics, weights,
  * gates and their gradients fp32.  LBN_ERR_UNSUPPORTED beyond 2^26 features, or 2^32 columns
  * (column_offset included). */
 #define LBN_NORM_NONE 0

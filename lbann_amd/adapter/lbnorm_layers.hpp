@@ -1343,7 +1343,9 @@ public:
   const Mat* branch = nullptr;          // the block's output
   const Mat* residual = nullptr;        // the stream before it (may stay null)
   const Mat32* gate = nullptr;          // one column per width / gate->Width() columns (may stay null)
-  Mat* new_residual = nullptr;          // h; backward reads it
+  // h.  With an output norm backward reads it: until then nothing may write over it, so in training a
+  // layer behind this one that takes it as `residual` needs a new_residual of its own.
+  Mat* new_residual = nullptr;
   Mat* output = nullptr;                // y; null without an output norm
   const Mat* output_gradient = nullptr;        // dL/dy; null without an output norm
   const Mat* new_residual_gradient = nullptr;  // dL/dh apart from y's part (may stay null with an output norm)

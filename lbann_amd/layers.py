@@ -16,6 +16,7 @@ path is done by torch, and there is no fallback when the library is missing.
 """
 import functools
 import operator
+import weakref
 
 import numpy as np
 import torch
@@ -246,11 +247,15 @@ class _Layer:
     def forward(self, x, in_place=False):
         self.bind_forward(x, in_place)
         self.fp_compute()
+        if in_place:
+            _wrote_over(x)
         return self.activations
 
     def backward(self, dy, in_place=False):
         self.bind_backward(dy, in_place)
         self.bp_compute()
+        if in_place:
+            _wrote_over(dy)
         return self.error_signals
 
 
@@ -843,6 +848,38 @@ def _same_kind(like, height, width, **matrices):
                              f"{height} x {width} {dtype} on {t.device}")
 
 
+def _share_memory(a, b):
+    """Whether two matrices have an entry in common.  Rows of one buffer that lie beside each other have none; of
+    matrices with different leading dimensions only the extents are looked at."""
+    if not (a.width and a.height and b.width and b.height):
+        return False
+    size_a, size_b = a.tensor.element_size(), b.tensor.element_size()
+    ld_a, ld_b = a.ldim * size_a, b.ldim * size_b
+    rows_a, rows_b = a.height * size_a, b.height * size_b
+    ahead = b.tensor.data_ptr() - a.tensor.data_ptr()
+    if not -((b.width - 1) * ld_b + rows_b) < ahead < (a.width - 1) * ld_a + rows_a:
+        return False
+    if ld_a != ld_b or a.width == 1 or b.width == 1:
+        return True
+    columns, rows = divmod(ahead, ld_a)  # b starts `rows` bytes into the column `columns` of a
+    return (rows < rows_a and -b.width < columns < a.width) or (rows + rows_b > ld_a and -b.width < columns + 1 < a.width)
+
+
+_SAVED = {}  # by id: residual norm layers (weak references) whose backward has matrices of the last forward to read
+
+
+def _wrote_over(m, by=None):
+    """A call (of the layer `by`) has written over its input m: backward of the layers that still read that memory is
+    refused from here on."""
+    for key, ref in list(_SAVED.items()):
+        layer = ref()
+        if layer is None or layer is by:
+            continue
+        if any(saved is not None and _share_memory(saved, m) for saved in layer._read_by_backward()):
+            layer._overwritten = True
+            _SAVED.pop(key, None)
+
+
 def _stream_for(m):
     """The current stream, as an address.  Kernels go to the current device: refuse matrices of
     another one."""
@@ -989,7 +1026,7 @@ class residual_norm_layer(_Dropout):
                 if t.dim() != 1 or t.numel() != self.size:
                     raise ValueError(f"{name} has shape {tuple(t.shape)}; expected ({self.size},)")
         self.branch = self.h = self.gate = self.residual = self.activations = self.m_statistics = None
-        self.m_has_residual = False
+        self.m_has_residual = self._overwritten = False
         self.m_gate_gradient = self._scratch_for = None
         for _, attribute in self._gradients:
             setattr(self, attribute, None)
@@ -1011,12 +1048,17 @@ class residual_norm_layer(_Dropout):
 
     def forward(self, branch, residual=None, gate=None, training=True, offset=None, in_place=False):
         """in_place: the new stream overwrites `residual`, and outside training, where no backward
-        needs it, y overwrites `branch`.  training=False: no dropout, no statistics."""
+        needs it, y overwrites `branch`.  training=False: no dropout, no statistics.
+
+        In training, `residual` must not be what another layer's backward is still to read: a layer with an
+        output norm reads the stream that it returned.  A layer whose matrices were written over refuses backward."""
         n, w, kinds, wt = self.size, branch.width, self._kinds, self.weights
         _same_kind(branch, n, w, branch=branch, residual=residual)
         stream = _stream_for(branch)
         self._check_weights(branch)
         self._check_gate(gate, branch)
+        if in_place:
+            self._check_places(branch, residual, gate, training)
         self._start(training, offset)
         self.branch, self.gate, self.m_has_residual = branch, gate, residual is not None
         h = residual if in_place and residual is not None else _matrix_beside(branch, n, w)
@@ -1031,7 +1073,38 @@ class residual_norm_layer(_Dropout):
             *_buffer(h), *_buffer(y), *_buffer(self.m_statistics))
         self.h = self.residual = h
         self.activations = y
+        self._keep(training)
+        if in_place and _SAVED:
+            if residual is not None:
+                _wrote_over(residual, self)
+            if y is branch:
+                _wrote_over(branch, self)
         return y
+
+    def _check_places(self, branch, residual, gate, training):
+        """Two outputs, or one and what is read again after it was written, need memory of their own."""
+        again = training and (self._kinds[0] or gate is not None)  # backward reads the branch
+        y_too = not training and self._kinds[1]                    # y takes the branch's place
+        o = branch.tensor.data_ptr() if branch.width else None
+        r = None if residual is None else residual.tensor.data_ptr()
+        clash = o is not None and o == r and (again or y_too)
+        if gate is not None and branch.width and (training or gate.width < branch.width):
+            clash = clash or gate.tensor.data_ptr() in (r, o if y_too else None)
+        if clash:
+            raise ValueError("in_place: branch, residual and gate need memory of their own")
+
+    def _keep(self, training):
+        self._overwritten = False
+        key = id(self)
+        if not training:
+            _SAVED.pop(key, None)
+        elif key not in _SAVED:
+            _SAVED[key] = weakref.ref(self, lambda _: _SAVED.pop(key, None))
+
+    def _read_by_backward(self):
+        """The matrices of the last forward (or bind_saved) that backward reads."""
+        branch = self.branch if self._kinds[0] or self.gate is not None else None
+        return branch, self.h if self._kinds[1] else None, self.gate
 
     def bind_saved(self, branch, h, statistics, gate=None, has_residual=True, offset=0, training=True):
         """What an earlier forward left behind, for a backward without one in this object
@@ -1042,6 +1115,7 @@ class residual_norm_layer(_Dropout):
         self.branch, self.h, self.m_statistics, self.gate = branch, h, statistics, gate
         self.residual, self.m_has_residual = h, bool(has_residual)
         self._start(training, offset)
+        self._keep(True)
 
     def backward(self, dy=None, dresidual=None):
         like = dy if dy is not None else dresidual
@@ -1049,6 +1123,8 @@ class residual_norm_layer(_Dropout):
             raise ValueError("backward takes dy exactly if there is an output norm, and dresidual if there is none")
         if self.m_statistics is None:
             raise ValueError("backward needs a training-mode forward (or bind_saved) first")
+        if self._overwritten:
+            raise ValueError("a later call with in_place has overwritten the stream, branch or gate that backward reads")
         n, w, kinds, wt, gate = self.size, like.width, self._kinds, self.weights, self.gate
         _same_kind(like, n, w, dy=dy, dresidual=dresidual, branch=self.branch, h=self.h)
         st = self.m_statistics
@@ -1137,6 +1213,8 @@ class logits_adjust_layer:
             _device_values(presence, w, torch.float32, "presence", x),
             _device_values(frequency, w, torch.float32, "frequency", x), bt, ld_bt, bv, ld_bv, biases, mk, ld_mk,
             0 if mask is None else mask.width, _device_values(mask_index, w, torch.int32, "mask_index", x))
+        if in_place:
+            _wrote_over(x)
         self.activations = y
         return y
 
