@@ -817,7 +817,7 @@ int lbn_residual_norm_fwd_bf16(lbn_stream_t stream, int64_t size, int64_t width,
  * caller whose share of a mini-batch may be empty clears these sums itself.
  * The workspace is lbn_residual_norm_bwd_workspace_bytes() large, 16-byte aligned:
  * has_weight_grads != 0 if any of the four weight gradients is wanted, num_gate_grads =
- * num_gates if dgate is, else 0, elem_bytes 4 or 2 for the storage type. */
+ * num_gates if dgate is, else 0, elem_bytes 4 or 2 for the storage type; 0 for sizes that backward refuses. */
 size_t lbn_residual_norm_bwd_workspace_bytes(int64_t size, int64_t width, int has_weight_grads,
                                              int64_t num_gate_grads, int elem_bytes);
 int lbn_residual_norm_bwd_f32(lbn_stream_t stream, int64_t size, int64_t width, int branch_norm,

@@ -1,0 +1,29 @@
+"""The size query of the residual norm's backward: any numbers, also those that the call itself refuses."""
+import pytest
+
+
+def size(*args):
+    from lbann_amd import capi
+    return capi.lib().lbn_residual_norm_bwd_workspace_bytes(*args)
+
+
+@pytest.mark.parametrize("n,width,gates", [(100, 4, 8), (100, 1, 2), (4096, 512, 513), (16, 6, 4), (16, 6, 2 ** 40), (20000, 3, 7)])
+@pytest.mark.parametrize("weights", [0, 1])
+def test_gates_that_do_not_divide_the_width(n, width, gates, weights):
+    """More gates than columns once divided by zero, which ends the process."""
+    assert size(n, width, weights, gates, 4) == 0
+
+
+def test_sizes_beyond_the_limits():
+    assert size(2 ** 26 + 1, 4, 1, 0, 2) == 0 and size(2 ** 62, 2 ** 62, 1, 0, 2) == 0
+    assert size(64, 2 ** 32 + 1, 1, 0, 2) == 0 and size(64, 2 ** 62, 1, 2, 2) == 0
+    assert size(2 ** 26, 4, 1, 0, 2) > 0 and size(64, 2 ** 32, 1, 0, 2) > 0
+    assert size(-1, 4, 1, 0, 2) == 0 and size(4, -1, 1, 0, 2) == 0 and size(4, 4, 1, -1, 2) == 0
+
+
+def test_gates_that_do():
+    for n in (1, 7, 64, 1000, 4096, 20000):
+        for width in (1, 6, 300, 7200):
+            for gates in (1, 2, 3, width):
+                if width % gates == 0:
+                    assert size(n, width, 1, gates, 4) >= size(n, width, 1, 0, 4) * (gates == 1) and size(n, width, 0, gates, 2) >= 16 * width
