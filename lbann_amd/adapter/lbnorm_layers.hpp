@@ -1294,9 +1294,16 @@ public:
 
   void fp_compute()
   {
+    const dropout_state before = state;
     state.start(is_training);
-    run(detail::pick<storage_of<T>::value>(lbn_dropout_fwd_f32, lbn_dropout_fwd_f16, lbn_dropout_fwd_bf16),
-        *io.prev_activations, *io.activations, "dropout_layer::fp_compute");
+    try {
+      run(detail::pick<storage_of<T>::value>(lbn_dropout_fwd_f32, lbn_dropout_fwd_f16, lbn_dropout_fwd_bf16),
+          *io.prev_activations, *io.activations, "dropout_layer::fp_compute");
+    }
+    catch (...) {
+      state = before;  // backward still repeats the last forward
+      throw;
+    }
   }
   void bp_compute()
   {

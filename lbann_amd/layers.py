@@ -942,6 +942,13 @@ class _Dropout:
             self.m_offset = int(offset) & 0xFFFFFFFFFFFFFFFF
         self.m_kept = self.m_keep_prob if training else 1.0
 
+    def _started(self):
+        """What _start changes, for a call that is refused after it: backward then still repeats the last forward."""
+        return self.m_offset, self.m_kept, self._next
+
+    def _restore(self, state):
+        self.m_offset, self.m_kept, self._next = state
+
     def _drop_args(self, like):
         step = None
         if self.m_step is not None:
@@ -960,8 +967,13 @@ class dropout_layer(_Layer, _Dropout):
         self.m_kept = self.m_keep_prob
 
     def forward(self, x, in_place=False, training=True, offset=None):
+        before = self._started()
         self._start(training, offset)
-        return super().forward(x, in_place)
+        try:
+            return super().forward(x, in_place)
+        except Exception:
+            self._restore(before)
+            raise
 
     def bind_forward(self, x, in_place=False):
         self.prev_activations = x
@@ -1059,18 +1071,24 @@ class residual_norm_layer(_Dropout):
         self._check_gate(gate, branch)
         if in_place:
             self._check_places(branch, residual, gate, training)
-        self._start(training, offset)
-        self.branch, self.gate, self.m_has_residual = branch, gate, residual is not None
         h = residual if in_place and residual is not None else _matrix_beside(branch, n, w)
         y = None
         if kinds[1]:
             y = branch if in_place and not training else _matrix_beside(branch, n, w)
-        self.m_statistics = _matrix_beside(branch, 4, w, torch.float32) if training else None
-        _entry("lbn_residual_norm_fwd", branch.tensor.dtype)(
-            stream, n, w, *kinds, self.m_epsilon, self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch),
-            *_buffer(residual), *_buffer(gate), 0 if gate is None else gate.width, _pointer(wt["branch_scale"]),
-            _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch),
-            *_buffer(h), *_buffer(y), *_buffer(self.m_statistics))
+        statistics = _matrix_beside(branch, 4, w, torch.float32) if training else None
+        before = self._started()
+        self._start(training, offset)
+        try:
+            _entry("lbn_residual_norm_fwd", branch.tensor.dtype)(
+                stream, n, w, *kinds, self.m_epsilon, self.m_residual_multiplier, self.m_branch_multiplier, *_buffer(branch),
+                *_buffer(residual), *_buffer(gate), 0 if gate is None else gate.width, _pointer(wt["branch_scale"]),
+                _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch),
+                *_buffer(h), *_buffer(y), *_buffer(statistics))
+        except Exception:
+            self._restore(before)
+            raise
+        # only now: a call that was refused leaves the last one's matrices, statistics and dropout together
+        self.branch, self.gate, self.m_has_residual, self.m_statistics = branch, gate, residual is not None, statistics
         self.h = self.residual = h
         self.activations = y
         self._keep(training)

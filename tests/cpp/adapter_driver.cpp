@@ -634,6 +634,26 @@ int drv_stale_statistics(void)
   return missed;
 }
 
+// A dropout forward that is refused leaves the offsets as they were.
+int drv_refused_dropout(void)
+{
+  int missed = 0;
+  device_matrix<float> a, b;
+  a.Attach(0, 6, nullptr, 1), b.Attach(0, 5, nullptr, 1);
+  dropout_layer<> l(0.5, 3);
+  l.io.prev_activations = &a, l.io.activations = &a;
+  l.fp_compute();
+  l.fp_compute();
+  if (l.state.offset != 1 || l.state.next_offset != 2 || l.state.kept != 0.5) ++missed;
+  l.io.activations = &b;
+  for (bool training : {true, false}) {
+    l.is_training = training;
+    try { l.fp_compute(); ++missed; } catch (const exception&) {}
+    if (l.state.offset != 1 || l.state.next_offset != 2 || l.state.kept != 0.5) ++missed;
+  }
+  return missed;
+}
+
 int drv_error_cases(void)
 {
   int missed = 0;
