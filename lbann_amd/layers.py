@@ -1039,7 +1039,8 @@ class residual_norm_layer(_Dropout):
                     raise ValueError(f"{name} has shape {tuple(t.shape)}; expected ({self.size},)")
         self.branch = self.h = self.gate = self.residual = self.activations = self.m_statistics = None
         self.m_has_residual = self._overwritten = False
-        self.m_gate_gradient = self._scratch_for = None
+        self.m_gate_gradient = None
+        self._scratch = None, 0  # a shape of backward and the scratch it takes
         for _, attribute in self._gradients:
             setattr(self, attribute, None)
 
@@ -1172,11 +1173,10 @@ class residual_norm_layer(_Dropout):
                 if m is not None:
                     m.tensor.zero_()
         key = w, gates, like.tensor.dtype, wanted > 0
-        if self._scratch_for != key:
-            self._scratch_for = key
-            self._scratch_bytes = capi.lib().lbn_residual_norm_bwd_workspace_bytes(
-                n, w, int(wanted > 0), gates, like.tensor.element_size())
-        need = self._scratch_bytes
+        last, need = self._scratch  # replaced as one, so that a thread beside this one sees both or neither
+        if last != key:
+            need = capi.lib().lbn_residual_norm_bwd_workspace_bytes(n, w, int(wanted > 0), gates, like.tensor.element_size())
+            self._scratch = key, need
         # scratch of this call alone: nothing that another stream or a recorded graph could share
         ws = like.tensor.new_empty((need,), dtype=torch.uint8) if need else None
         _entry("lbn_residual_norm_bwd", like.tensor.dtype)(

@@ -27,3 +27,34 @@ def test_gates_that_do():
             for gates in (1, 2, 3, width):
                 if width % gates == 0:
                     assert size(n, width, 1, gates, 4) >= size(n, width, 1, 0, 4) * (gates == 1) and size(n, width, 0, gates, 2) >= 16 * width
+
+
+def test_size_kept_by_a_layer_while_another_thread_asks(monkeypatch):
+    """A call that comes between the size query of another and its use gets the size of its own shape."""
+    from lbann_amd import layers as L
+    made, inside = [], []
+
+    class Library:
+        @staticmethod
+        def lbn_residual_norm_bwd_workspace_bytes(n, width, *rest):
+            if width not in inside:   # as another thread would, at the worst moment
+                inside.append(width)
+                backward(width)
+            return 1000 + width
+
+    monkeypatch.setattr(L.capi, "lib", lambda: Library)
+    monkeypatch.setattr(L, "_stream_for", lambda m: 0)
+    monkeypatch.setattr(L, "_entry", lambda name, dtype: lambda *args: made.append((args[2], args[-1])))
+    layer = L.residual_norm_layer(8, device="cpu")
+
+    def matrix(width, height=8):
+        return L.DeviceMatrix(height, width, device="cpu", fill=1.0)
+
+    def backward(width):
+        layer.bind_saved(matrix(width), matrix(width), matrix(width, 4))
+        layer.backward(matrix(width), matrix(width))
+
+    for width in (5, 9, 5):
+        backward(width)
+    assert len(made) == 5 and all(need == 1000 + width for width, need in made), made
+    L._SAVED.clear()
