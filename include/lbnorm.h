@@ -880,10 +880,10 @@ int lbn_residual_norm_bwd_bf16(lbn_stream_t stream, int64_t size, int64_t width,
  * A grammar that allows nothing leaves a column of -infinity, on which the softmax layers
  * return NaN: end such a sequence first.  x and y may be the same matrix.  No workspace.
  * Storage fp32, IEEE binary16 or bfloat16, fp32 arithmetic, one rounding.
- * LBN_ERR_UNSUPPORTED beyond some 2^31 entries or tokens or 2^23 sequences (fewer where the
- * vocabulary takes several workgroups), or where one 32-bit word
- * cannot hold a count up to max_tokens, a place in the bias list and one bit more (131072 tokens
- * leave room for 8191 biases). */
+ * LBN_ERR_UNSUPPORTED from a vocabulary, a width, a history or a bias list of some 2^31 on; where ceil(vocabulary / s)
+ * times width reaches w, with s = 2048 and w = 2^23 for max_tokens below 1024, s = 8192 and w = 2^22 below 4096, s =
+ * 16384 and w = 2^21 from there on; or where one 32-bit word cannot hold a count up to max_tokens, a place in the bias
+ * list and one bit more (131072 tokens leave room for 8191 biases). */
 int lbn_logits_adjust_f32(lbn_stream_t stream, int64_t vocabulary, int64_t width, const float* x,
                           int64_t ldx, float* y, int64_t ldy, const int32_t* tokens, int64_t ld_tokens,
                           int64_t max_tokens, const int32_t* lengths, const int32_t* prompt_lengths,
