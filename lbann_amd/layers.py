@@ -247,14 +247,14 @@ class _Layer:
     def forward(self, x, in_place=False):
         self.bind_forward(x, in_place)
         self.fp_compute()
-        if in_place:
+        if in_place and _SAVED:
             _wrote_over(x)
         return self.activations
 
     def backward(self, dy, in_place=False):
         self.bind_backward(dy, in_place)
         self.bp_compute()
-        if in_place:
+        if in_place and _SAVED:
             _wrote_over(dy)
         return self.error_signals
 
@@ -942,13 +942,6 @@ class _Dropout:
             self.m_offset = int(offset) & 0xFFFFFFFFFFFFFFFF
         self.m_kept = self.m_keep_prob if training else 1.0
 
-    def _started(self):
-        """What _start changes, for a call that is refused after it: backward then still repeats the last forward."""
-        return self.m_offset, self.m_kept, self._next
-
-    def _restore(self, state):
-        self.m_offset, self.m_kept, self._next = state
-
     def _drop_args(self, like):
         step = None
         if self.m_step is not None:
@@ -967,12 +960,12 @@ class dropout_layer(_Layer, _Dropout):
         self.m_kept = self.m_keep_prob
 
     def forward(self, x, in_place=False, training=True, offset=None):
-        before = self._started()
+        before = self.m_offset, self.m_kept, self._next
         self._start(training, offset)
         try:
             return super().forward(x, in_place)
         except Exception:
-            self._restore(before)
+            self.m_offset, self.m_kept, self._next = before  # backward still repeats the last forward
             raise
 
     def bind_forward(self, x, in_place=False):
@@ -1077,7 +1070,7 @@ class residual_norm_layer(_Dropout):
         if kinds[1]:
             y = branch if in_place and not training else _matrix_beside(branch, n, w)
         statistics = _matrix_beside(branch, 4, w, torch.float32) if training else None
-        before = self._started()
+        before = self.m_offset, self.m_kept, self._next
         self._start(training, offset)
         try:
             _entry("lbn_residual_norm_fwd", branch.tensor.dtype)(
@@ -1086,13 +1079,14 @@ class residual_norm_layer(_Dropout):
                 _pointer(wt["branch_bias"]), _pointer(wt["output_scale"]), _pointer(wt["output_bias"]), *self._drop_args(branch),
                 *_buffer(h), *_buffer(y), *_buffer(statistics))
         except Exception:
-            self._restore(before)
+            self.m_offset, self.m_kept, self._next = before  # backward still repeats the last forward
             raise
         # only now: a call that was refused leaves the last one's matrices, statistics and dropout together
         self.branch, self.gate, self.m_has_residual, self.m_statistics = branch, gate, residual is not None, statistics
         self.h = self.residual = h
         self.activations = y
-        self._keep(training)
+        if not training or self._overwritten or id(self) not in _SAVED:
+            self._keep(training)
         if in_place and _SAVED:
             if residual is not None:
                 _wrote_over(residual, self)
@@ -1231,7 +1225,7 @@ class logits_adjust_layer:
             _device_values(presence, w, torch.float32, "presence", x),
             _device_values(frequency, w, torch.float32, "frequency", x), bt, ld_bt, bv, ld_bv, biases, mk, ld_mk,
             0 if mask is None else mask.width, _device_values(mask_index, w, torch.int32, "mask_index", x))
-        if in_place:
+        if in_place and _SAVED:
             _wrote_over(x)
         self.activations = y
         return y
