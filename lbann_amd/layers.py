@@ -124,13 +124,13 @@ _STORAGE = {torch.float32: "f32", torch.float16: "f16", torch.float64: "f64"}
 def _storage(owner, types, *matrices):
     """Suffix of the entry points for the storage type that every matrix of a call has (None: no such matrix).  A type
     that the layer has no kernels for, bfloat16 among them, is refused: read as another type it would reach past its end."""
-    kinds = {m.tensor.dtype for m in matrices if m is not None}
+    kinds = {m.dtype for m in matrices if m is not None}
     if len(kinds) != 1:
         raise TypeError(f"{type(owner).__name__}: matrices of different types {sorted(map(str, kinds))}")
     suffix = _STORAGE.get(kinds.pop())
     if suffix not in types:
         raise TypeError(f"{type(owner).__name__}: storage is {' or '.join(types)}, not "
-                        f"{next(m.tensor.dtype for m in matrices if m is not None)}")
+                        f"{next(m.dtype for m in matrices if m is not None)}")
     return suffix
 
 
@@ -1112,7 +1112,7 @@ class residual_norm_layer(_Dropout):
         if not training:
             _SAVED.pop(key, None)
         elif key not in _SAVED:
-            _SAVED[key] = weakref.ref(self, lambda _: _SAVED.pop(key, None))
+            _SAVED[key] = weakref.ref(self, lambda _, saved=_SAVED: saved.pop(key, None))
 
     def _read_by_backward(self):
         """The matrices of the last forward (or bind_saved) that backward reads."""
