@@ -145,6 +145,15 @@ constexpr int64_t kRnStreamBytes = int64_t(256) << 20;
 
 constexpr int64_t kRnMostFeatures = int64_t(1) << 26;  // the merge of partial rows has a workgroup for 64 of them
 
+// Whether a call takes the kernels for whole units and epsilons that leave no subnormal sum.  The others are for any
+// length and epsilon (4096 x 8192 bf16 between two RMS norms with a gate without an epsilon: forward 45.7 us instead of
+// 48.0, backward 108 instead of 77).
+template <typename ARGS>
+static bool rn_even(const ARGS& a)
+{
+  return a.n % 8 == 0 && (a.epsilon >= kRnNormalEpsilon || (a.branch_norm == kNormNone && a.output_norm == kNormNone));
+}
+
 static unsigned ld32(int64_t ld) { return static_cast<unsigned>(ld); }
 
 // Leading dimensions (0 for a matrix that is not there) and widths that the row kernels' 32-bit indices hold.
@@ -235,7 +244,7 @@ static RnBwdPlan rn_bwd_plan(int64_t n, int64_t width, int weight_grads, int64_t
   return p;
 }
 
-// The row kernel of a call.  Lengths that are no multiple of eight with a gate take the one that accumulates
+// The row kernel of a call.  Calls that are not `even` (rn_even) take, with a gate, the one that accumulates
 // everything (without a gate that costs: 502 x 12100 bf16, two norms, 24.5 us against 19.3).
 template <typename T, int TEAM>
 static auto rn_bwd_kernel(bool norm, bool gate, bool bias, bool even, bool stream) -> void (*)(RnBwdRows<T>)
@@ -255,7 +264,7 @@ static auto rn_bwd_kernel(bool norm, bool gate, bool bias, bool even, bool strea
 template <typename T>
 static auto rn_bwd_kernel(const RnBwdArgs<T>& g, const RnShape& shape, bool bias) -> void (*)(RnBwdRows<T>)
 {
-  const bool norm = g.branch_norm != kNormNone, gate = g.gate != nullptr, even = g.n % 8 == 0;
+  const bool norm = g.branch_norm != kNormNone, gate = g.gate != nullptr, even = rn_even(g);
   const int64_t bytes = g.n * g.width * static_cast<int64_t>(sizeof(T)) * (1 + 2 * !!g.dy + !!g.dh + !!g.branch + !!g.dresidual);
   const bool stream = stream_call_inputs(bytes, kRnStreamBytes);
   if (shape.sub) return rn_bwd_kernel<T, 16>(norm, gate, bias, even, stream);
@@ -337,7 +346,7 @@ static int rn_fwd(lbn_stream_t stream, RnFwdArgs<T> a, int64_t num_gates, double
   if (shape.v && rn_fits32(a.width, {a.ld_branch, a.residual ? a.ld_residual : 0, a.gate ? a.ld_gate : 0, a.h ? a.ld_h : 0,
                                    a.y ? a.ld_y : 0, a.stats ? a.ld_stats : 0})) {
     const int64_t bytes = a.n * a.width * static_cast<int64_t>(sizeof(T)) * (1 + !!a.residual + !!a.h + !!a.y);
-    if (a.n % 8) rn_launch_fwd<T, false, false>(st, a, shape);
+    if (!rn_even(a)) rn_launch_fwd<T, false, false>(st, a, shape);
     else if (stream_call_inputs(bytes, kRnStreamBytes)) rn_launch_fwd<T, true, true>(st, a, shape);
     else rn_launch_fwd<T, true, false>(st, a, shape);
   }

@@ -377,7 +377,7 @@ rn_fwd_rows(RnFwdRows<T> a)
       float mean1 = 0.f, var1 = 1.f, mean2 = 0.f, var2 = 1.f;
       if (a.branch_norm != kNormNone) {
         row_moments<V, SUB, kFull, EVEN>(x, share, a.branch_norm, team.inv_n, team.inv_mine, merge, mean1, var1);
-        const float rstd = rn_rstd(var1 + a.epsilon);
+        const float rstd = rn_rstd<!EVEN>(var1 + a.epsilon);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if constexpr (!kKeepWeights) {
@@ -410,7 +410,7 @@ rn_fwd_rows(RnFwdRows<T> a)
       }
       if (a.output_norm != kNormNone) {
         row_moments<V, SUB, kFull, EVEN>(x, share, a.output_norm, team.inv_n, team.inv_mine, merge, mean2, var2);
-        const float rstd = rn_rstd(var2 + a.epsilon);
+        const float rstd = rn_rstd<!EVEN>(var2 + a.epsilon);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           if constexpr (!kKeepWeights) {
@@ -442,7 +442,8 @@ constexpr int kMergeRows = 3;
 // gate in registers.  At the end of the range, and for several gates at the end of each gate's
 // columns, the teams' sums are merged through LDS and leave one partial row.
 // BRANCH_NORM, GATE, BIAS: what there is to accumulate (BIAS: of any norm); GATE and BIAS may be
-// set where there is none.  EVEN: the length is a multiple of eight.  STREAM: inputs past the caches.
+// set where there is none.  EVEN: the length is a multiple of eight and the epsilon a normal number.  STREAM: inputs
+// past the caches.
 //
 // Entries that do not exist are loaded as zeros and have zero weights, so that they add nothing
 // to any sum and need no masks.
@@ -615,8 +616,8 @@ rn_bwd_rows(RnBwdRows<T> a)
       const bool active = col < end;
       float e[8], f[8], x[8];
       RnColumnStats s = qstats;
-      s.rstd1 = BRANCH_NORM ? rn_rstd(s.rstd1 + a.epsilon) : 1.f;
-      s.rstd2 = rn_rstd(s.rstd2 + a.epsilon);
+      s.rstd1 = BRANCH_NORM ? rn_rstd<!EVEN>(s.rstd1 + a.epsilon) : 1.f;
+      s.rstd2 = rn_rstd<!EVEN>(s.rstd2 + a.epsilon);
       float o[8];
       U::template widen<EVEN>(qy, shift, f);
       U::template widen<EVEN>(qs, shift, x);
