@@ -337,7 +337,8 @@ rn_bwd_long_sums(RnBwdArgs<T> a)
         load_weights8(a.output_scale, k, valid, 1.f, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float p = j < valid ? dy[j] * w[j] : 0.f;
+          if (j >= valid) continue;  // the distance of a missing entry from the mean may overflow
+          const float p = dy[j] * w[j];
           sp += p;
           spx = __builtin_fmaf(p, (x[j] - s.mean2) * s.rstd2, spx);
         }
@@ -356,7 +357,8 @@ rn_bwd_long_sums(RnBwdArgs<T> a)
         load_weights8(a.branch_scale, k, valid, 1.f, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float p = j < valid ? du[j] * w[j] : 0.f;
+          if (j >= valid) continue;
+          const float p = du[j] * w[j];
           sp += p;
           spu = __builtin_fmaf(p, uh[j], spu);
         }

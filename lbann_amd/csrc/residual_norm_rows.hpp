@@ -39,6 +39,8 @@ struct Unit {
     }
     return r;
   }
+  // ROUND: what leaves at the bottom comes back at the top, so that missing entries are entries of the column.
+  template <bool ROUND = false>
   static __device__ __forceinline__ raw_t moved(const raw_t& r, int shift)
   {
     constexpr int W = 2 * static_cast<int>(sizeof(T));  // words of a unit
@@ -46,19 +48,23 @@ struct Unit {
     __builtin_memcpy(d, &r, 4 * W);
     if constexpr (sizeof(T) == 2) {
       if (shift & 1) {
+        const uint32_t first = ROUND ? d[0] : 0u;
 #pragma unroll
-        for (int i = 0; i < W; ++i) d[i] = d[i] >> 16 | (i + 1 < W ? d[i + 1] << 16 : 0u);
+        for (int i = 0; i < W; ++i) d[i] = d[i] >> 16 | (i + 1 < W ? d[i + 1] : first) << 16;
       }
       shift >>= 1;
     }
 #pragma unroll
     for (int by = 1; by < W; by *= 2) {
       if (shift & by) {
+        uint32_t first[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) d[i] = i + by < W ? d[i + by] : 0u;
+        for (int i = 0; i < W; ++i) first[i] = ROUND ? d[i] : 0u;
+#pragma unroll
+        for (int i = 0; i < W; ++i) d[i] = i + by < W ? d[i + by] : first[i + by - W];
       }
     }
-    if (shift & W) {
+    if (!ROUND && (shift & W)) {
 #pragma unroll
       for (int i = 0; i < W; ++i) d[i] = 0u;
     }
@@ -81,6 +87,20 @@ struct Unit {
       r = moved(r, shift);
     }
     widen(r, v);
+  }
+  // For what a mean is taken from in backward.  A zero's distance from the mean may overflow when it is scaled (columns of one
+  // large number), and infinity times the zero that stands beside it is no zero.  So missing entries of partial units
+  // are entries of the column, which are as near to its mean as any; missing whole units: RowShare::epsilon.
+  template <bool EVEN>
+  static __device__ __forceinline__ void widen_centred(raw_t r, int shift, float (&v)[8])
+  {
+    if constexpr (EVEN) {
+      widen<true>(r, shift, v);
+    }
+    else {
+      if (shift) r = moved<true>(r, shift);
+      widen(r, v);
+    }
   }
   static __device__ __forceinline__ void widen(const raw_t& r, float (&v)[8])
   {
@@ -129,6 +149,9 @@ struct RowShare {
       shift[i] = 8 - valid[i];
     }
   }
+  // The epsilon of unit i.  Kernels for whole units: infinite where nothing exists, which makes 1 / sqrt(var + epsilon)
+  // zero there (see Unit::widen_centred).
+  __device__ __forceinline__ float epsilon(int i, float e) const { return !EVEN || valid[i] ? e : INFINITY; }
   // The thread's entries of a weight vector (null: `fill`); 0 where nothing exists.
   __device__ __forceinline__ void weights(const float* w, int i, float fill, float (&out)[8]) const
   {
@@ -377,9 +400,9 @@ rn_fwd_rows(RnFwdRows<T> a)
       float mean1 = 0.f, var1 = 1.f, mean2 = 0.f, var2 = 1.f;
       if (a.branch_norm != kNormNone) {
         row_moments<V, SUB, kFull, EVEN>(x, share, a.branch_norm, team.inv_n, team.inv_mine, merge, mean1, var1);
-        const float rstd = rn_rstd<!EVEN>(var1 + a.epsilon);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+          const float rstd = rn_rstd<!EVEN>(var1 + (kFull ? a.epsilon : share.epsilon(i, a.epsilon)));
           if constexpr (!kKeepWeights) {
             weights(a.branch_scale, i, 1.f, w1[0]);
             weights(a.branch_bias, i, 0.f, b1[0]);
@@ -387,7 +410,9 @@ rn_fwd_rows(RnFwdRows<T> a)
           constexpr bool kw = kKeepWeights;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            x[i][j] = __builtin_fmaf((x[i][j] - mean1) * rstd, w1[kw ? i : 0][j], b1[kw ? i : 0][j]);
+            // partial units: the weight first, which is zero where nothing exists
+            x[i][j] = EVEN ? __builtin_fmaf((x[i][j] - mean1) * rstd, w1[kw ? i : 0][j], b1[kw ? i : 0][j])
+                           : __builtin_fmaf(x[i][j] - mean1, rstd * w1[kw ? i : 0][j], b1[kw ? i : 0][j]);
         }
       }
 #pragma unroll
@@ -445,8 +470,8 @@ constexpr int kMergeRows = 3;
 // set where there is none.  EVEN: the length is a multiple of eight and the epsilon a normal number.  STREAM: inputs
 // past the caches.
 //
-// Entries that do not exist are loaded as zeros and have zero weights, so that they add nothing
-// to any sum and need no masks.
+// Entries that do not exist are loaded as zeros (partial units of what is normalised: as others of the column) and have
+// zero weights, so that they add nothing to any sum that is kept and need no masks.
 //
 // Bound by HBM: 4096 x 8192 bf16 between two RMS norms with a gate, 384 MiB moved, in 76.8 us (5.2
 // TB/s).  One workgroup a compute unit keeps the partial rows few (256 of them: 4.9 us to merge).
@@ -479,6 +504,7 @@ rn_bwd_rows(RnBwdRows<T> a)
   const bool several_gates = GATE && a.cols_per_gate < width;
   const bool output_norm = a.output_norm != kNormNone;
   const bool read_branch = BRANCH_NORM || (GATE && a.branch);
+  const float epsilon = share.epsilon(0, a.epsilon);
   unsigned first, last;
   rn_range(blockIdx.x, width, a.cols_per_range, a.cols_per_gate, a.ranges_per_gate, first, last);
 
@@ -616,13 +642,13 @@ rn_bwd_rows(RnBwdRows<T> a)
       const bool active = col < end;
       float e[8], f[8], x[8];
       RnColumnStats s = qstats;
-      s.rstd1 = BRANCH_NORM ? rn_rstd<!EVEN>(s.rstd1 + a.epsilon) : 1.f;
-      s.rstd2 = rn_rstd<!EVEN>(s.rstd2 + a.epsilon);
+      s.rstd1 = BRANCH_NORM ? rn_rstd<!EVEN>(s.rstd1 + epsilon) : 1.f;
+      s.rstd2 = rn_rstd<!EVEN>(s.rstd2 + epsilon);
       float o[8];
       U::template widen<EVEN>(qy, shift, f);
-      U::template widen<EVEN>(qs, shift, x);
+      U::template widen_centred<EVEN>(qs, shift, x);
       U::template widen<EVEN>(qh, shift, e);
-      U::template widen<EVEN>(qo, shift, o);
+      U::template widen_centred<EVEN>(qo, shift, o);
       // a single team carries the next column over the end of a gate's columns
       const unsigned next = col + teams;
       in_flight = teams == 1 && next < last;
