@@ -140,7 +140,8 @@ struct RnShape {
 
 // Calls that move this much read their inputs past the caches (4096 features, bf16, three sets of
 // matrices in turn: 256 MiB forward in 51.4 -> 48.4 us, 384 MiB backward in 89 -> 78 us, but 128 MiB forward in
-// 23 -> 25 us).
+// 23 -> 25 us; sizes between were not measured).  Lengths that are no multiple of eight never do: their kernels exist with
+// ordinary loads only.
 constexpr int64_t kRnStreamBytes = int64_t(256) << 20;
 
 constexpr int64_t kRnMostFeatures = int64_t(1) << 26;  // the merge of partial rows has a workgroup for 64 of them

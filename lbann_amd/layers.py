@@ -3,9 +3,10 @@ channelwise softmax; instance norm, entry-wise batch norm, cross entropy and the
 layers) and of the operators around a transformer's residual stream and logits (dropout,
 residual norm, logits adjustment), over the C ABI.
 
-Each class keeps the reference layer's constructor parameters, its member
+Each class of a reference layer keeps that layer's constructor parameters, its member
 matrices and its two compute hooks, `fp_compute()` and `bp_compute()`
-(include/lbann/layers/layer.hpp:835,852), and forwards them to liblbnorm.so.
+(include/lbann/layers/layer.hpp:835,852), and forwards them to liblbnorm.so; residual norm and
+logits adjustment, which have no layer there, have forward() and backward() only.
 A harness plays the role of data_type_layer::forward_prop / back_prop_impl_
 (src/layers/data_type_layer.cpp:170-275, :292-376): it binds the input
 matrices, sizes the outputs (left uninitialised, as the reference does) and
@@ -920,8 +921,11 @@ def _device_values(t, n, dtype, what, like):
 
 
 class _Dropout:
-    """Where the random bits of a layer's calls come from: key `seed`, counter `offset`.  Every
-    training-mode forward without an explicit offset takes the next one."""
+    """Where the random bits of a layer's calls come from: key `seed`, counter `offset`.  A
+    training-mode forward without an explicit offset takes the next one (0, 1, ...; explicit ones do not count).
+
+    The mask is a function of these numbers alone, so that another object with the same seed repeats it (recomputation,
+    other ranks).  Layers that are to drop independently need seeds of their own: the default is the same for all."""
 
     def __init__(self, keep_prob, seed):
         if not 0.0 < keep_prob <= 1.0:
