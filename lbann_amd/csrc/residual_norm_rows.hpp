@@ -322,7 +322,7 @@ __device__ __forceinline__ T* column(T* p, unsigned col, unsigned ld)
 }
 
 // Forward.  Bound by HBM where the columns fill the chip: 4096 x 8192 fp16 with dropout, 256 MiB moved,
-// in 48.9 us (5.5 TB/s; a copy reaches 5.1); 1151 x 3000 fp32 between two layer norms in 16.4 us (3.4
+// in 49.3 us (5.4 TB/s; a copy reaches 5.1); 1151 x 3000 fp32 between two layer norms in 16.1 us (3.4
 // TB/s: three rounds of columns a workgroup, of which the last is a third full).  A single column of 4096
 // takes 3.2 us, of which about 3 is what an empty launch traces at.  One resident wave of
 // workgroups walks the columns: with the weights in registers that beats workgroups of one, two or
